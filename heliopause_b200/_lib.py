@@ -49,6 +49,13 @@ SIGNATURES = {
     "hpc_topk_merge_keys": (_i, [_vp, _sz, _sz, _sz, C.c_float, _vp, _vp, _vp]),
     "hpc_sample_candidates": (_i, [_vp, _vp, _sz, _sz, C.c_double, C.c_double, _i, C.c_uint32, _vp, _vp, _sz,
                                    _sz, C.c_double, _vp, _vp]),
+    "hpc_paged_kv_append": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _i, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _i, C.c_double,
+                                 _vp, _vp, _i, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _vp]),
+    "hpc_attention_workspace_bytes": (_i, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "hpc_paged_attention": (_i, [_vp, _sz, _vp, _vp, _i, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
+                                 C.c_float, _sz, _vp, _sz, _vp, _i, _vp, _vp]),
+    "hpc_prompt_attention": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _i, _vp, _sz, _sz, _sz, _sz, _sz, _sz, C.c_float, _sz,
+                                  _vp, _sz, _vp, _i, _vp, _vp]),
     "hpc_model_create": (_i, [_vp, C.POINTER(_vp)]),
     "hpc_model_release": (_i, [_vp]),
     "hpc_model_set_weight": (_i, [_vp, _i, _i, _vp]),

@@ -21,6 +21,7 @@
 #include "hc_internal.h"
 #include "hc_kernels.cuh"
 #include "hc_lmhead.cuh"
+#include "hc_paged.cuh"
 
 thread_local std::string g_last_error;
 
@@ -104,6 +105,8 @@ int hpc_device_error(void) {
   if (v == 0) return HPC_OK;
   const int zero = 0;
   HPC_CK(cudaMemcpy(w, &zero, sizeof zero, cudaMemcpyHostToDevice), "clear device status");
+  if (v == hc::DEVICE_ERR_PAGE)
+    return fail(HPC_ERR_SHAPE, "a paged batch's table, lengths or starts pointed outside their buffers");
   return fail(HPC_ERR_TIMEOUT, "a kernel wait timed out on the device (code %d)", v);
 }
 

@@ -1,0 +1,856 @@
+// hc_paged_attn.cu -- attention of few query rows over a long cache.
+//
+//   o = sum_j softmax_j(scale * q . k_j) v_j  over the keys j <= pos of the
+// query's sequence (j > pos - window with a window), for the newest tokens of
+// every sequence: one (decode), a pending token and its drafts (verify), or
+// any number.  The query heads that share a KV head and the new tokens of the
+// sequence are the rows of one product, so each key and value is read once
+// for all of them: per element 2 rows multiply-adds for 2 bytes, which the
+// memory bounds by far up to 16 rows.
+//
+// Work: an item is (sequence, KV head, block of 8 or 16 rows); its keys are cut
+// into tiles of 64, and the tiles of all items, in order, are dealt out
+// evenly to a grid that fills the machine -- a CTA takes a run of tiles, so
+// ragged batches balance to a tile and one long sequence spreads over every
+// SM, with no plan made on the host.  A CTA that holds an item's every tile
+// writes its output; items cut by a CTA boundary leave a partial (running
+// maximum, sum, unnormalised output; at most two per CTA, in the workspace)
+// which hc_attn_join_kernel joins in tile order.
+//
+// CTA: a producer warp keeps a ring of K and V tiles full by TMA (page by
+// page, each piece of 64 elements 128-byte swizzled), so 100 KB and more are
+// in flight per SM whatever the warps compute.  Four consumer warps take 16
+// keys each of every tile and share nothing until the item ends: S^T = K Q^T
+// (m16n8k16: the 16 keys are the M side, so 8 rows cost 8 columns instead of
+// a padded 16), the row maxima and sums in f32 over the warp's own keys, P
+// rounded to the cache's type for the second product -- its relative 2^-9
+// (2^-12 for f16) is that of the values it multiplies -- and O^T += V^T P^T in
+// f32 registers.  The warps' four partials are added in shared memory at the end.
+//
+// A key that a row does not see adds nothing to it, whatever its value
+// holds: values at or behind the sequence's end are zeroed in shared memory
+// before they are multiplied (stale pages may hold NaN), and where a tile has
+// keys that only some rows see, a value that is not finite sends the warp
+// through scalar sums over the visible pairs.
+#include <algorithm>
+#include <atomic>
+
+#include "hc_paged.cuh"
+
+namespace hc {
+namespace {
+
+constexpr int AR_TILE = 64;      // keys per tile
+constexpr int AR_WARPS = 4;      // consumer warps, 16 keys of a tile each
+constexpr int AR_THREADS = 32 * (AR_WARPS + 1);
+constexpr float LN2 = 0.6931471805599453f;
+
+template <int D, int NB>
+struct RowsCfg {
+  static constexpr int kSlot = AR_TILE * D * 2;                          // one K or V tile
+  static constexpr int kMergeRow = D + 4;                                // floats; + 4: no bank conflicts
+  static constexpr int kMerge = AR_WARPS * 8 * NB * kMergeRow * 4;
+  // as many tiles in flight as fit beside the merge buffer with 1 / 2 / 3 CTAs per SM
+  static constexpr int kSlots = D == 256 ? (NB == 1 ? 6 : 5) : D == 128 ? (NB == 1 ? 5 : 4) : (NB == 1 ? 8 : 6);
+  static constexpr int kSmem = 1024 + kSlots * kSlot + kMerge;           // + alignment
+};
+
+// What the join kernel needs of an item cut by a CTA boundary.
+struct JoinRec {
+  int seq, head, block;  // block < 0: nothing to join
+  int last;              // last CTA that holds tiles of it
+  long long total;       // tiles of the launch
+};
+
+struct RowsWork {
+  float* o;      // [2 * grid][8 NB][D]
+  float2* ml;    // [2 * grid][8 NB]: maximum (in log2 units), sum
+  JoinRec* rec;  // [grid]
+};
+
+struct RowsArgs {
+  AttnArgs a;
+  PagedBatch b;
+  RowsWork w;
+  int box_rows;  // rows of one TMA copy: min(page_size, 64), 64 without pages
+  int64_t slots; // rows of the tensor maps (a coordinate there reads zeros)
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Tiles of one sequence's items: [first, first + count), the same for its
+// heads and row blocks (a block skips those it does not see); at least one,
+// so that rows that see nothing are written too.
+struct SeqTiles {
+  int first, count, blocks;
+};
+template <int NB>
+__device__ __forceinline__ SeqTiles seq_tiles(const SeqSpan& q, int group, int window) {
+  SeqTiles t;
+  const int low = window > 0 ? max(0, q.len - q.n - window + 1) : 0;
+  t.first = low / AR_TILE;
+  t.count = max(1, (q.len + AR_TILE - 1) / AR_TILE - t.first);
+  t.blocks = (q.n * group + 8 * NB - 1) / (8 * NB);
+  return t;
+}
+
+__device__ __forceinline__ long long cta_begin(long long total, int c, int grid) { return total * c / grid; }
+
+// The keys [lo, hi) that some row of an item's block sees.
+struct BlockSpan {
+  int rows, lo, hi, pos0;
+};
+template <int NB>
+__device__ __forceinline__ BlockSpan block_span(const SeqSpan& q, int block, int group, int window) {
+  BlockSpan s;
+  const int r0 = block * 8 * NB;
+  s.rows = min(8 * NB, q.n * group - r0);
+  s.pos0 = q.len - q.n;  // position of the sequence's first new token
+  const int p_first = s.pos0 + r0 / group, p_last = s.pos0 + (r0 + s.rows - 1) / group;
+  s.lo = window > 0 ? max(0, p_first - window + 1) : 0;
+  s.hi = min(q.len, p_last + 1);
+  return s;
+}
+
+// A run of tiles [u, end) walked item by item.
+struct Walk {
+  int s, head, block, tile;  // tile: within the item, 0 ..
+  long long u, end;
+};
+
+template <class T>
+__device__ __forceinline__ bool not_finite2(uint32_t v);
+template <>
+__device__ __forceinline__ bool not_finite2<__half>(uint32_t v) {
+  return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u;
+}
+template <>
+__device__ __forceinline__ bool not_finite2<__nv_bfloat16>(uint32_t v) {
+  return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+}
+
+template <class T, int D, int NB>
+__global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
+    hc_attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const __grid_constant__ RowsArgs p) {
+  using Cfg = RowsCfg<D, NB>;
+  constexpr int R = 8 * NB, KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[Cfg::kSlots], empty[Cfg::kSlots];
+  __shared__ long long s_sum[AR_WARPS + 1];
+  __shared__ Walk s_walk;
+  __shared__ float2 s_ml[AR_WARPS][R];
+  const int t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
+  const int grid = int(gridDim.x), cta = int(blockIdx.x);
+  const int group = p.a.heads / p.a.kv_heads, window = p.a.window;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  float* merge = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + Cfg::kSlots * Cfg::kSlot);
+  if (t == 0) {
+    for (int i = 0; i < Cfg::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], AR_WARPS);
+    }
+  }
+  pdl_launch_next();
+  pdl_wait_prior();
+
+  // ---- this CTA's run of tiles: thread t counts sequences [t * per, ...)
+  const int per = (p.b.seqs + AR_THREADS - 1) / AR_THREADS;
+  long long mine = 0;
+  bool any_bad = false;
+  for (int i = 0; i < per; ++i) {
+    const int s = t * per + i;
+    if (s >= p.b.seqs) break;
+    bool bad;
+    const SeqSpan q = seq_span(p.b, s, &bad);
+    any_bad = any_bad || bad;
+    const SeqTiles st = seq_tiles<NB>(q, group, window);
+    mine += (long long)p.a.kv_heads * st.blocks * st.count;
+  }
+  if (any_bad && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  if (t == 0) p.w.rec[cta].block = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i <= AR_WARPS; ++i) {
+    if (i < warp) incl += s_sum[i];
+    total += s_sum[i];
+  }
+  const long long u0 = cta_begin(total, cta, grid), u1 = cta_begin(total, cta + 1, grid);
+  if (u0 >= u1) return;
+  if (incl - mine <= u0 && u0 < incl) {
+    long long at = incl - mine;
+    for (int s = t * per;; ++s) {
+      bool bad;
+      const SeqTiles st = seq_tiles<NB>(seq_span(p.b, s, &bad), group, window);
+      const long long n = (long long)p.a.kv_heads * st.blocks * st.count;
+      if (u0 < at + n) {
+        const long long d = u0 - at;
+        Walk w;
+        w.s = s;
+        w.tile = int(d % st.count);
+        w.block = int(d / st.count % st.blocks);
+        w.head = int(d / st.count / st.blocks);
+        w.u = u0;
+        w.end = u1;
+        s_walk = w;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Walk w = s_walk;
+
+  int it = 0;  // K and V tiles so far: slot it % kSlots, phase it / kSlots
+  bool ok = true;
+  if (warp == AR_WARPS) {
+    // ---- producer: lane i copies the tile's i-th page
+    const int box = p.box_rows, ppt = AR_TILE / box;
+    while (w.u < w.end && ok) {
+      bool bad;
+      const SeqSpan q = seq_span(p.b, w.s, &bad);
+      const SeqTiles st = seq_tiles<NB>(q, group, window);
+      for (; w.head < p.a.kv_heads && w.u < w.end && ok; ++w.head, w.block = 0) {
+        for (; w.block < st.blocks && w.u < w.end && ok; ++w.block, w.tile = 0) {
+          const BlockSpan sp = block_span<NB>(q, w.block, group, window);
+          for (; w.tile < st.count && w.u < w.end && ok; ++w.tile, ++w.u) {
+            const int k0 = (st.first + w.tile) * AR_TILE;
+            if (k0 + AR_TILE <= sp.lo || k0 >= sp.hi) continue;
+            const int copies = (min(AR_TILE, q.len - k0) + box - 1) / box;
+            int row = 0;
+            if (lane < ppt && lane < copies) {
+              if (p.b.table) {
+                const int key = k0 + lane * box;
+                const int page = p.b.table[int64_t(w.s) * p.b.width + (key >> p.b.page_shift)];
+                const bool in = page >= 0 && page < p.b.pages;
+                if (!in && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
+                row = in ? int((int64_t(page) << p.b.page_shift) + (key & ((1 << p.b.page_shift) - 1))) : int(p.slots);
+              } else {
+                row = q.row0 + k0;
+              }
+            }
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv, ++it) {
+              const int slot = it % Cfg::kSlots, ph = it / Cfg::kSlots;
+              if (ph > 0 && !mbar_wait_parity_sleep(&empty[slot], uint32_t(ph - 1) & 1u, p.a.err)) ok = false;
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              if (lane == 0) mbar_expect_tx(&full[slot], uint32_t(copies * box * D * 2));
+              __syncwarp();
+              if (lane < copies)
+                tma_load_3d(base + slot * Cfg::kSlot + lane * box * D * 2, kv ? &vmap : &kmap, 0, row,
+                            w.head * (D / 64), smem_u32(&full[slot]));
+            }
+          }
+        }
+        if (w.block < st.blocks) break;
+      }
+      if (w.head < p.a.kv_heads) break;
+      ++w.s, w.head = 0, w.block = 0, w.tile = 0;
+    }
+    // nothing of this CTA's is in flight when it ends: the consumers wait
+    // for every copy; after a timeout the copies issued are waited for here
+    if (!ok)
+      for (int i = max(0, it - Cfg::kSlots); i < it; ++i)
+        mbar_wait_parity_sleep(&full[i % Cfg::kSlots], uint32_t(i / Cfg::kSlots) & 1u, p.a.err);
+    return;
+  }
+
+  // ---- consumers
+  const int lr = lane >> 2, lc = lane & 3;
+  const int box_shift = __ffs(p.box_rows) - 1;
+  // byte offset of key row j of a tile (its first 128-byte piece); pieces are box_rows * 128 apart
+  const auto row_off = [&](int j) { return (j >> box_shift) * (p.box_rows * D * 2) + (j & (p.box_rows - 1)) * 128; };
+  const int piece = p.box_rows * 128;
+  // this lane's ldmatrix rows (fixed within the tile) and 16-byte chunks
+  const int kj = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
+  const int vj = warp * 16 + (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
+  const uint32_t koff = uint32_t(row_off(kj)), voff = uint32_t(row_off(vj));
+  while (w.u < w.end) {
+    bool bad;
+    const SeqSpan q = seq_span(p.b, w.s, &bad);
+    const SeqTiles st = seq_tiles<NB>(q, group, window);
+    for (; w.head < p.a.kv_heads && w.u < w.end; ++w.head, w.block = 0) {
+      for (; w.block < st.blocks && w.u < w.end; ++w.block, w.tile = 0) {
+        const BlockSpan sp = block_span<NB>(q, w.block, group, window);
+        const int r0 = w.block * R;
+        // B fragments of Q^T, straight from the rows
+        uint32_t qf[NB][KS][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int r = r0 + nb * 8 + lr;
+          const bool in = r - r0 < sp.rows;
+          const T* src = static_cast<const T*>(p.a.q) + int64_t(q.row0 + (in ? r / group : 0)) * p.a.q_stride +
+                         (w.head * group + (in ? r % group : 0)) * D + lc * 2;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            qf[nb][k][0] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+            qf[nb][k][1] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
+          }
+        }
+        // keys [low, lim] of this lane's two rows of every 8
+        int lim[NB][2], low[NB][2];
+        float m[NB][2], l[NB][2];
+        float o[NB][KS][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = nb * 8 + lc * 2 + e;
+            const int pos = sp.pos0 + (r0 + r) / group;
+            lim[nb][e] = r < sp.rows ? min(pos, q.len - 1) : -1;
+            low[nb][e] = window > 0 ? pos - window + 1 : 0;
+            m[nb][e] = -INFINITY;
+            l[nb][e] = 0.0f;
+          }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nb][k][e] = 0.0f;
+        // every key of [all_lo, all_hi] is seen by every row of the block
+        const int all_hi = min(q.len - 1, sp.pos0 + r0 / group);
+        const int all_lo = window > 0 ? sp.pos0 + (r0 + sp.rows - 1) / group - window + 1 : 0;
+        const int tile0 = w.tile;
+        for (; w.tile < st.count && w.u < w.end; ++w.tile, ++w.u) {
+          const int k0 = (st.first + w.tile) * AR_TILE;
+          // after a wait gave up the warp only walks on, to meet the others at the barriers
+          if (!ok || k0 + AR_TILE <= sp.lo || k0 >= sp.hi) continue;
+          const int j0 = k0 + warp * 16;  // this warp's keys
+          const bool idle = j0 >= sp.hi || j0 + 16 <= sp.lo;
+          const int ks = it % Cfg::kSlots, kph = it / Cfg::kSlots;
+          const int vs = (it + 1) % Cfg::kSlots, vph = (it + 1) / Cfg::kSlots;
+          it += 2;
+          uint32_t pb[NB][2];
+          float pr[NB][4];
+          ok = mbar_wait_parity(&full[ks], uint32_t(kph) & 1u, p.a.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) continue;
+          if (!idle) {
+            float s[2][NB][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[h][nb][e] = 0.0f;
+            const uint32_t kb = base + ks * Cfg::kSlot + koff;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              uint32_t af[4];
+              ldsm4(af, kb + (k >> 2) * piece + ((((k & 3) * 2 + kc) ^ (kj & 7)) << 4));
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma16<T>(s[k & 1][nb], af, qf[nb][k][0], qf[nb][k][1]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[ks]);
+            bool grew = false;
+            float corr[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int ja = j0 + lr, jb = ja + 8;
+                float a = (s[0][nb][e] + s[1][nb][e]) * p.a.scale_log2;
+                float b = (s[0][nb][2 + e] + s[1][nb][2 + e]) * p.a.scale_log2;
+                a = ja <= lim[nb][e] && ja >= low[nb][e] ? a : -INFINITY;
+                b = jb <= lim[nb][e] && jb >= low[nb][e] ? b : -INFINITY;
+                float mx = fmaxf(a, b);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[nb][e], mx);
+                const float ms = mn == -INFINITY ? 0.0f : mn;
+                corr[nb][e] = ex2(m[nb][e] - ms);
+                grew = grew || mn != m[nb][e];
+                m[nb][e] = mn;
+                pr[nb][e] = ex2(a - ms);
+                pr[nb][2 + e] = ex2(b - ms);
+                l[nb][e] = l[nb][e] * corr[nb][e] + (pr[nb][e] + pr[nb][2 + e]);
+              }
+              // [key][row] quarters -> [row][key], the B fragment of the second product
+              pb[nb][0] = transpose8(HalfOps<T>::pack(pr[nb][0], pr[nb][1]));
+              pb[nb][1] = transpose8(HalfOps<T>::pack(pr[nb][2], pr[nb][3]));
+            }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[nb][k][e] *= corr[nb][e & 1];
+            }
+          } else {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[ks]);
+          }
+          ok = mbar_wait_parity(&full[vs], uint32_t(vph) & 1u, p.a.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) continue;
+          if (!idle) {
+            const uint32_t vt = base + vs * Cfg::kSlot;
+            bool scalar = false;
+            if (j0 + 15 > all_hi || j0 < all_lo) {  // some row does not see some of these keys
+              bool odd = false;
+              for (int i = lane; i < 16 * (D / 8); i += 32) {
+                const int jj = i / (D / 8), c = i % (D / 8), j = warp * 16 + jj;
+                const uint32_t at = vt + row_off(j) + (c >> 3) * piece + (((c & 7) ^ (j & 7)) << 4);
+                if (j0 + jj >= q.len) {
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
+                } else {
+                  uint32_t v0, v1, v2, v3;
+                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                               : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3)
+                               : "r"(at)
+                               : "memory");
+                  odd = odd || not_finite2<T>(v0) || not_finite2<T>(v1) || not_finite2<T>(v2) || not_finite2<T>(v3);
+                }
+              }
+              // the zeros are read by ldmatrix, and the slot's next copy
+              // (the async proxy) must come after them
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              scalar = __any_sync(0xffffffffu, odd);
+              __syncwarp();
+            }
+            if (!scalar) {
+#pragma unroll
+              for (int k = 0; k < KS; ++k) {
+                uint32_t af[4];
+                ldsm4_t(af, vt + voff + (k >> 2) * piece + ((((k & 3) * 2 + vc) ^ (vj & 7)) << 4));
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma16<T>(o[nb][k], af, pb[nb][0], pb[nb][1]);
+              }
+            } else {
+              for (int jj = 0; jj < 16; ++jj) {
+                const int j = j0 + jj;
+                if (j >= q.len) break;
+                const int rj = warp * 16 + jj;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float pe = __shfl_sync(0xffffffffu, jj < 8 ? pr[nb][e] : pr[nb][2 + e], (jj & 7) * 4 + lc);
+                    if (j > lim[nb][e] || j < low[nb][e]) continue;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                      for (int h = 0; h < 2; ++h) {
+                        const int d = k * 16 + h * 8 + lr;
+                        uint16_t bits;
+                        asm volatile("ld.shared.u16 %0, [%1];"
+                                     : "=h"(bits)
+                                     : "r"(vt + row_off(rj) + (d >> 6) * piece + ((((d >> 3) & 7) ^ (rj & 7)) << 4) +
+                                           (d & 7) * 2)
+                                     : "memory");
+                        const float v = HalfOps<T>::unpack(bits).x;
+                        o[nb][k][h * 2 + e] = fmaf(pe, v, o[nb][k][h * 2 + e]);
+                      }
+                  }
+                }
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[vs]);
+        }
+        // ---- the item (or this CTA's part of it) is done: add the warps up
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = l[nb][e];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            if (lr == 0) s_ml[warp][nb * 8 + lc * 2 + e] = make_float2(m[nb][e], v);
+          }
+        float* mb = merge + warp * R * Cfg::kMergeRow;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mb[(nb * 8 + lc * 2 + (e & 1)) * Cfg::kMergeRow + k * 16 + (e >> 1) * 8 + lr] = o[nb][k][e];
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * AR_WARPS) : "memory");
+        const bool whole = tile0 == 0 && w.tile == st.count;
+        const int part = tile0 > 0 ? 2 * cta : 2 * cta + 1;
+        constexpr int TPR = 32 * AR_WARPS / R;  // threads per row
+        {
+          const int r = t / TPR, c = t % TPR;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < AR_WARPS; ++i) mx = fmaxf(mx, s_ml[i][r].x);
+          const float ms = mx == -INFINITY ? 0.0f : mx;
+          float f[AR_WARPS], sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < AR_WARPS; ++i) {
+            f[i] = ex2(s_ml[i][r].x - ms);
+            sum += f[i] * s_ml[i][r].y;
+          }
+          if (r < sp.rows) {
+            const int row = q.row0 + (r0 + r) / group, head = w.head * group + (r0 + r) % group;
+            const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            for (int d = c * 4; d < D; d += TPR * 4) {
+              float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+              for (int i = 0; i < AR_WARPS; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(merge + (i * R + r) * Cfg::kMergeRow + d);
+                v.x += f[i] * x.x, v.y += f[i] * x.y, v.z += f[i] * x.z, v.w += f[i] * x.w;
+              }
+              if (whole) {
+                const int64_t at = (int64_t(row) * p.a.heads + head) * D + d;
+                if (p.a.out_f32)
+                  *reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + at) =
+                      make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                else
+                  *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + at) =
+                      make_uint2(HalfOps<T>::pack(v.x * inv, v.y * inv), HalfOps<T>::pack(v.z * inv, v.w * inv));
+              } else {
+                *reinterpret_cast<float4*>(p.w.o + (int64_t(part) * R + r) * D + d) = v;
+              }
+            }
+            if (c == 0) {
+              if (!whole) p.w.ml[part * R + r] = make_float2(mx, sum);
+              else if (p.a.lse) p.a.lse[int64_t(row) * p.a.heads + head] = sum == 0.0f ? -INFINITY : LN2 * (mx + log2f(sum));
+            }
+          }
+        }
+        if (t == 0 && !whole && tile0 == 0) {
+          // this CTA holds the item's first tile: it records the join
+          JoinRec r;
+          r.seq = w.s, r.head = w.head, r.block = w.block;
+          const long long last_tile = w.u - w.tile + st.count - 1;
+          r.last = int(((last_tile + 1) * grid - 1) / total);
+          r.total = total;
+          p.w.rec[cta] = r;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * AR_WARPS) : "memory");
+      }
+      if (w.block < st.blocks) break;
+    }
+    if (w.head < p.a.kv_heads) break;
+    ++w.s, w.head = 0, w.block = 0, w.tile = 0;
+  }
+}
+
+// Joins the partials of the item whose first tile CTA blockIdx.x held, one
+// row per block: the maximum of all, then the sums in CTA order.
+template <class T, int D, int NB>
+__global__ void __launch_bounds__(D / 2) hc_attn_join_kernel(const __grid_constant__ RowsArgs p, int grid) {
+  constexpr int R = 8 * NB, TH = D / 2;
+  __shared__ float s_max[TH / 32], s_f[TH];
+  __shared__ int s_part[TH];
+  const int c0 = int(blockIdx.x), r = int(blockIdx.y), t = int(threadIdx.x);
+  pdl_wait_prior();
+  const JoinRec rec = p.w.rec[c0];
+  if (rec.block < 0) return;
+  bool bad;
+  const SeqSpan q = seq_span(p.b, rec.seq, &bad);
+  const int group = p.a.heads / p.a.kv_heads;
+  const int r0 = rec.block * R;
+  if (r >= min(R, q.n * group - r0)) return;
+  const auto part_of = [&](int c) { return c == c0 ? 2 * c + 1 : 2 * c; };
+  const auto held = [&](int c) { return cta_begin(rec.total, c, grid) < cta_begin(rec.total, c + 1, grid); };
+  float mx = -INFINITY;
+  for (int c = c0 + t; c <= rec.last; c += TH)
+    if (held(c)) mx = fmaxf(mx, p.w.ml[part_of(c) * R + r].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if ((t & 31) == 0) s_max[t >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < TH / 32; ++i) mx = fmaxf(mx, s_max[i]);
+  const float ms = mx == -INFINITY ? 0.0f : mx;
+  float sum = 0.0f, x = 0.0f, y = 0.0f;
+  for (int b = c0; b <= rec.last; b += TH) {
+    __syncthreads();
+    const int c = b + t;
+    if (c <= rec.last) {
+      float f = 0.0f;
+      int part = -1;
+      if (held(c)) {
+        part = part_of(c);
+        const float2 v = p.w.ml[part * R + r];
+        f = ex2(v.x - ms);
+        // summed below in CTA order by every thread alike
+      }
+      s_f[t] = f;
+      s_part[t] = part;
+    }
+    __syncthreads();
+    const int n = min(TH, rec.last - b + 1);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const int part = s_part[i];
+      if (part < 0) continue;
+      const float f = s_f[i];
+      const float2 v = *reinterpret_cast<const float2*>(p.w.o + (int64_t(part) * R + r) * D + 2 * t);
+      sum += f * p.w.ml[part * R + r].y;
+      x += f * v.x;
+      y += f * v.y;
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  const int64_t row = int64_t(q.row0 + (r0 + r) / group) * p.a.heads + rec.head * group + (r0 + r) % group;
+  if (p.a.out_f32)
+    *reinterpret_cast<float2*>(static_cast<float*>(p.a.out) + row * D + 2 * t) = make_float2(x * inv, y * inv);
+  else
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.a.out) + row * D + 2 * t) = HalfOps<T>::pack(x * inv, y * inv);
+  if (t == 0 && p.a.lse) p.a.lse[row] = sum == 0.0f ? -INFINITY : LN2 * (mx + log2f(sum));
+}
+
+// CTAs per SM times the SMs, of which the workspace allows for 160.
+constexpr int kMaxSms = 160;
+constexpr int ctas_per_sm(int dim) { return dim == 256 ? 1 : dim == 128 ? 2 : 3; }
+
+size_t ws_bytes(int grid, int rows, int dim) {
+  const auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
+  return al(size_t(2 * grid) * rows * dim * 4) + al(size_t(2 * grid) * rows * 8) + al(size_t(grid) * sizeof(JoinRec));
+}
+
+template <class T, int D, int NB>
+cudaError_t launch_rows(RowsArgs& p, const KvSource& kv, void* workspace, cudaStream_t st) {
+  using Cfg = RowsCfg<D, NB>;
+  auto kernel = hc_attn_rows_kernel<T, D, NB>;
+  static std::atomic<uint64_t> attr{0};
+  cudaError_t e = once_per_current_device(attr, [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  const int grid = std::min(kMaxSms, sm_count()) * ctas_per_sm(D);
+  const auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.w.o = reinterpret_cast<float*>(ws);
+  ws += al(size_t(2 * grid) * 8 * NB * D * 4);
+  p.w.ml = reinterpret_cast<float2*>(ws);
+  ws += al(size_t(2 * grid) * 8 * NB * 8);
+  p.w.rec = reinterpret_cast<JoinRec*>(ws);
+  p.box_rows = p.b.table ? std::min(AR_TILE, 1 << p.b.page_shift) : AR_TILE;
+  p.slots = int64_t(kv.slots);
+  CUtensorMap km, vm;
+  e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, p.box_rows, D / 64);
+  if (e == cudaSuccess)
+    e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, p.box_rows, D / 64);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kernel, dim3(grid), dim3(AR_THREADS), Cfg::kSmem, st, km, vm, p);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(hc_attn_join_kernel<T, D, NB>, dim3(grid, 8 * NB), dim3(D / 2), 0, st, p, grid);
+}
+
+template <class T, int D>
+cudaError_t launch_rows_d(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_t st) {
+  // 8 rows hold a group of up to 8 heads at one token each; more new tokens
+  // or a larger group fill 16, which halves the times the keys are read
+  return int64_t(p.a.max_q) * (p.a.heads / p.a.kv_heads) <= 8 ? launch_rows<T, D, 1>(p, kv, ws, st)
+                                                              : launch_rows<T, D, 2>(p, kv, ws, st);
+}
+
+template <class T>
+cudaError_t launch_rows_t(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_t st) {
+  switch (p.a.dim) {
+    case 64: return launch_rows_d<T, 64>(p, kv, ws, st);
+    case 128: return launch_rows_d<T, 128>(p, kv, ws, st);
+    default: return launch_rows_d<T, 256>(p, kv, ws, st);
+  }
+}
+
+}  // namespace
+
+size_t attn_rows_workspace_bytes(int heads, int kv_heads, int dim) {
+  (void)heads, (void)kv_heads;
+  return ws_bytes(kMaxSms * ctas_per_sm(dim), 16, dim);
+}
+
+cudaError_t launch_attn_rows(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
+                             cudaStream_t st) {
+  RowsArgs p{};
+  p.a = a;
+  p.b = b;
+  return kv.dtype == HPC_DTYPE_F16 ? launch_rows_t<__half>(p, kv, workspace, st)
+                                   : launch_rows_t<__nv_bfloat16>(p, kv, workspace, st);
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (the
+// library does not link the driver library itself).
+cudaError_t encode_kv_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t slots,
+                          uint64_t stride, int heads, int dim, int box_rows, int box_pieces) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> cached{nullptr};
+  Encode encode = cached.load();
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess) return e;
+    if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorSymbolNotFound;
+    encode = reinterpret_cast<Encode>(fn);
+    cached.store(encode);
+  }
+  const cuuint64_t dims[3] = {64, slots, cuuint64_t(heads) * (dim / 64)};
+  const cuuint64_t strides[2] = {stride * 2, 128};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(box_pieces)};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = encode(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+}  // namespace hc
+
+int hpc_paged_check(const char* what, size_t heads, size_t kv_heads, size_t head_dim, size_t rows, size_t seqs,
+                    size_t pages, size_t page_size, size_t table_width) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return hpc_fail(HPC_ERR_SHAPE, "%s: head_dim %zu (64, 128 or 256)", what, head_dim);
+  if (kv_heads < 1 || heads < 1 || heads % kv_heads || heads > 1024)
+    return hpc_fail(HPC_ERR_HEADS, "%s: %zu heads over %zu KV heads", what, heads, kv_heads);
+  if (rows > size_t(INT32_MAX) || seqs > (1u << 20))
+    return hpc_fail(HPC_ERR_SHAPE, "%s: %zu rows of %zu sequences", what, rows, seqs);
+  if (page_size) {
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+      return hpc_fail(HPC_ERR_SHAPE, "%s: page_size %zu (a power of two from 16 to 1024)", what, page_size);
+    if (pages < 1 || pages > (size_t(INT32_MAX) - 1024) / page_size || table_width < 1 ||
+        table_width > size_t(INT32_MAX) / page_size)
+      return hpc_fail(HPC_ERR_SHAPE, "%s: %zu pages, a table of %zu", what, pages, table_width);
+  }
+  return HPC_OK;
+}
+
+hc::PagedBatch hpc_paged_batch(const int32_t* starts, const int32_t* lens, const int32_t* table, size_t seqs,
+                               size_t width, size_t rows, size_t pages, size_t page_size) {
+  hc::PagedBatch b{};
+  b.starts = starts;
+  b.kv_lens = lens;
+  b.table = table;
+  b.seqs = int(seqs);
+  b.width = int(width);
+  b.rows = int(rows);
+  while (page_size > 1) ++b.page_shift, page_size >>= 1;
+  b.pages = int64_t(pages);
+  return b;
+}
+
+namespace {
+
+int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSource& kv, hc::PagedBatch b,
+              size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale, size_t window,
+              void* d_workspace, size_t workspace_bytes, void* d_out, int out_dtype, float* d_lse, void* stream) {
+  if (kv.dtype != HPC_DTYPE_F16 && kv.dtype != HPC_DTYPE_BF16)
+    return hpc_fail(HPC_ERR_TYPE, "%s: keys and values of type %d", what, kv.dtype);
+  if (out_dtype != HPC_DTYPE_F32 && out_dtype != kv.dtype)
+    return hpc_fail(HPC_ERR_TYPE, "%s: output type %d", what, out_dtype);
+  if (q_stride < heads * head_dim || q_stride % 8 || q_stride > size_t(INT32_MAX) || kv.k_stride < kv_heads * head_dim ||
+      kv.k_stride % 8 || kv.v_stride < kv_heads * head_dim || kv.v_stride % 8 || kv.k_stride > size_t(INT32_MAX) ||
+      kv.v_stride > size_t(INT32_MAX))
+    return hpc_fail(HPC_ERR_SHAPE, "%s: row strides %zu, %zu, %zu (multiples of 8)", what, q_stride,
+                    size_t(kv.k_stride), size_t(kv.v_stride));
+  if (window > size_t(INT32_MAX) || !(scale == scale))
+    return hpc_fail(HPC_ERR_SHAPE, "%s: window %zu, scale %g", what, window, double(scale));
+  if (b.rows == 0 || b.seqs == 0) return HPC_OK;
+  if (!d_q || !kv.k || !kv.v || !b.starts || !d_out || !d_workspace) return hpc_fail(HPC_ERR_ARG, "null pointer");
+  const auto off = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+  if (off(d_q) || off(kv.k) || off(kv.v) || off(d_out) || off(d_workspace))
+    return hpc_fail(HPC_ERR_ARG, "%s: tensors must be aligned to 16 bytes", what);
+  const size_t need = hc::attn_rows_workspace_bytes(int(heads), int(kv_heads), int(head_dim));
+  if (workspace_bytes < need)
+    return hpc_fail(HPC_ERR_SHAPE, "%s: a workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  hc::AttnArgs a{};
+  a.q = d_q;
+  a.q_stride = int64_t(q_stride);
+  a.out = d_out;
+  a.lse = d_lse;
+  a.heads = int(heads), a.kv_heads = int(kv_heads), a.dim = int(head_dim);
+  a.window = int(window);
+  a.scale_log2 = float(double(scale) * 1.4426950408889634);
+  a.out_f32 = out_dtype == HPC_DTYPE_F32;
+  a.max_q = int(std::min(max_query_len, size_t(b.rows)));
+  a.err = hc::device_status_word();
+  HPC_CK(hc::launch_attn_rows(a, b, kv, d_workspace, static_cast<cudaStream_t>(stream)), what);
+  return HPC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hpc_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t head_dim, size_t *out_bytes) {
+  if (int rc = hpc_paged_check("attention workspace", heads, kv_heads, head_dim, 0, 0, 0, 0, 0)) return rc;
+  if (!out_bytes) return hpc_fail(HPC_ERR_ARG, "null pointer");
+  *out_bytes = hc::attn_rows_workspace_bytes(int(heads), int(kv_heads), int(head_dim));
+  return HPC_OK;
+}
+
+int hpc_paged_attention(const void *d_q, size_t q_stride, const void *d_key_cache, const void *d_value_cache,
+                        int cache_dtype, size_t pages, size_t page_size, const int32_t *d_page_table,
+                        size_t table_width, const int32_t *d_query_starts, const int32_t *d_kv_lens, size_t seqs,
+                        size_t rows, size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale,
+                        size_t window, void *d_workspace, size_t workspace_bytes, void *d_out, int out_dtype,
+                        float *d_lse, void *stream) {
+  if (page_size == 0) return hpc_fail(HPC_ERR_SHAPE, "paged attention: page_size 0");
+  if (int rc = hpc_paged_check("paged attention", heads, kv_heads, head_dim, rows, seqs, pages, page_size, table_width))
+    return rc;
+  if (rows && seqs && (!d_page_table || !d_kv_lens)) return hpc_fail(HPC_ERR_ARG, "null pointer");
+  const uint64_t stride = uint64_t(kv_heads) * head_dim;
+  const hc::KvSource kv{d_key_cache, d_value_cache, uint64_t(pages) * page_size, stride, stride, cache_dtype};
+  return attention("paged attention", d_q, q_stride, kv,
+                   hpc_paged_batch(d_query_starts, d_kv_lens, d_page_table, seqs, table_width, rows, pages, page_size),
+                   heads, kv_heads, head_dim, max_query_len, scale, window, d_workspace, workspace_bytes, d_out,
+                   out_dtype, d_lse, stream);
+}
+
+int hpc_prompt_attention(const void *d_q, size_t q_stride, const void *d_k, size_t k_stride, const void *d_v,
+                         size_t v_stride, int dtype, const int32_t *d_query_starts, size_t seqs, size_t rows,
+                         size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale,
+                         size_t window, void *d_workspace, size_t workspace_bytes, void *d_out, int out_dtype,
+                         float *d_lse, void *stream) {
+  if (int rc = hpc_paged_check("prompt attention", heads, kv_heads, head_dim, rows, seqs, 0, 0, 0)) return rc;
+  const hc::KvSource kv{d_k, d_v, rows, k_stride, v_stride, dtype};
+  return attention("prompt attention", d_q, q_stride, kv,
+                   hpc_paged_batch(d_query_starts, nullptr, nullptr, seqs, 0, rows, 0, 0), heads, kv_heads, head_dim,
+                   max_query_len, scale, window, d_workspace, workspace_bytes, d_out, out_dtype, d_lse, stream);
+}
+
+}  // extern "C"

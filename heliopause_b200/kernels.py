@@ -23,6 +23,7 @@ then part of the call, as it is for the WASM linear-memory copies).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -340,3 +341,214 @@ def set_matmul_order(exact: bool) -> None:
 def device_error() -> None:
     """Raises CudaKernelError(ERR_TIMEOUT) if a kernel's bounded wait gave up."""
     assert_cuda_ok(_lib.lib().hpc_device_error(), "deviceStatus")
+
+
+# ---- serving many sequences: paged KV cache and its attention ---------------------
+
+_DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _check_i32(name: str, device: torch.device, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+            raise CudaKernelError(ERR_ARG, f"{name}: starts, lengths and page tables are contiguous int32 tensors on "
+                                           f"{device}")
+
+
+def _rows3(name: str, t: torch.Tensor, device: torch.device, heads: int, dim: int) -> torch.Tensor:
+    """[rows][heads][dim] on `device`, heads and elements contiguous within a row."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: [rows][{heads}][{dim}] on {device}, not {tuple(t.shape)} on {t.device}")
+    st = t.stride()
+    if st[2] != 1 or (st[1] != dim and heads > 1) or st[0] % 8 or st[0] < heads * dim or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.stride(0) != heads * dim:  # a single row keeps any stride
+            t = t.as_strided(t.shape, (heads * dim, dim, 1))
+    return t
+
+
+def _check_cache(name: str, key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: key and value caches are [pages][page_size][kv_heads][head_dim]")
+    if not (key_cache.is_cuda and key_cache.device == value_cache.device and key_cache.is_contiguous()
+            and value_cache.is_contiguous()):
+        raise CudaKernelError(ERR_ARG, f"{name}: the caches are contiguous tensors on one device")
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                    page_table: torch.Tensor, query_starts: torch.Tensor, kv_lens: torch.Tensor, *,
+                    q: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+                    q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, norm_v: bool = False,
+                    eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """New tokens into a paged KV cache (hpc_paged_kv_append): per-head RMS
+    norms, the NeoX rotation by position * inv_freq (f64) and the write into
+    each token's page, in place; returns the queries normed and rotated in
+    the cache's type (q_out, or a new tensor), or None without q.
+
+    k, v, q: [rows][heads][head_dim], f32 or the cache's type, views with a
+    row stride allowed.  key_cache, value_cache: [pages][page_size][kv_heads]
+    [head_dim].  Sequence s owns rows query_starts[s] .. query_starts[s+1];
+    kv_lens[s] is its length with them; its token j lies in page
+    page_table[s][j // page_size].  Rows behind the last sequence are left."""
+    name = "pagedKvAppend"
+    _check_cache(name, key_cache, value_cache)
+    pages, page_size, kv_heads, dim = key_cache.shape
+    dev, dt = key_cache.device, key_cache.dtype
+    _check_i32(name, dev, page_table, query_starts, kv_lens)
+    seqs = kv_lens.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or query_starts.numel() != seqs + 1:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {seqs} sequences, a table of {tuple(page_table.shape)}, "
+                                         f"{query_starts.numel()} starts")
+    k = _rows3(name, k, dev, kv_heads, dim)
+    v = _rows3(name, v, dev, kv_heads, dim)
+    rows, heads = k.shape[0], kv_heads
+    if v.shape[0] != rows or v.dtype != k.dtype:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: keys and values differ in rows or type")
+    if dt not in _DTYPE_IDS or k.dtype not in _DTYPE_IDS:
+        raise CudaKernelError(ERR_TYPE, f"{name}: {k.dtype} into a cache of {dt}")
+    qp = qs = op = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != rows or q.dtype != k.dtype:
+            raise CudaKernelError(ERR_SHAPE, f"{name}: queries and keys differ in rows or type")
+        heads = q.shape[1]
+        q = _rows3(name, q, dev, heads, dim)
+        if q_out is None:
+            q_out = torch.empty((rows, heads, dim), dtype=dt, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype != dt or q_out.device != dev or not q_out.is_contiguous():
+            raise CudaKernelError(ERR_SHAPE, f"{name}: q_out is contiguous {tuple(q.shape)} of {dt}")
+        qp, qs, op = q.data_ptr(), q.stride(0), q_out.data_ptr()
+    half = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous():
+            raise CudaKernelError(ERR_ARG, f"{name}: inv_freq is a contiguous float64 tensor on {dev}")
+        half = inv_freq.numel()
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != dim or w.device != dev or not w.is_contiguous()):
+            raise CudaKernelError(ERR_ARG, f"{name}: norm weights are {dim} contiguous float32 values on {dev}")
+    with _on_device(dev):
+        code = _lib.lib().hpc_paged_kv_append(
+            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), qp, qs, _DTYPE_IDS[k.dtype], rows, heads, kv_heads, dim,
+            inv_freq.data_ptr() if half else None, half, q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, int(norm_v), eps, key_cache.data_ptr(),
+            value_cache.data_ptr(), _DTYPE_IDS[dt], pages, page_size, page_table.data_ptr(), page_table.shape[1],
+            query_starts.data_ptr(), kv_lens.data_ptr(), seqs, op, _raw_stream(dev))
+    if code:
+        assert_cuda_ok(code, name)
+    return q_out if q is not None else None
+
+
+class _on_device:
+    """Makes `device` current for a call when another one is."""
+    __slots__ = ("index", "back")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        cur = torch._C._cuda_getDevice()
+        self.back = cur if cur != self.index else -1
+        if self.back >= 0:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back >= 0:
+            torch.cuda.set_device(self.back)
+
+
+@functools.lru_cache(maxsize=None)
+def _attention_workspace(heads: int, kv_heads: int, dim: int) -> int:
+    n = C.c_size_t()
+    assert_cuda_ok(_lib.lib().hpc_attention_workspace_bytes(heads, kv_heads, dim, C.byref(n)), "attentionWorkspace")
+    return n.value
+
+
+def _attention_out(name, q, out, out_dtype, return_lse):
+    dt = out.dtype if out is not None else out_dtype or q.dtype
+    if out is None:
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
+        raise CudaKernelError(ERR_SHAPE, f"{name}: out is contiguous {tuple(q.shape)} on {q.device}")
+    if dt not in _DTYPE_IDS:
+        raise CudaKernelError(ERR_TYPE, f"{name}: output of {dt}")
+    lse = torch.full(q.shape[:2], -torch.inf, dtype=torch.float32, device=q.device) if return_lse else None
+    return out, lse
+
+
+def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
+                    query_starts: torch.Tensor, kv_lens: torch.Tensor, *, max_query_len: int, scale: float,
+                    window: int = 0, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                    return_lse: bool = False):
+    """Causal attention of every sequence's newest rows over its pages
+    (hpc_paged_attention): decode (one row each), verify, or chunks of
+    prompts.  Arguments as paged_kv_append's; window > 0: a row sees that
+    many keys, itself included.  max_query_len: the most rows of a sequence.
+    Returns [rows][heads][head_dim] (and the log-sum-exp [rows][heads] with
+    return_lse)."""
+    name = "pagedAttention"
+    _check_cache(name, key_cache, value_cache)
+    pages, page_size, kv_heads, dim = key_cache.shape
+    dev, dt = key_cache.device, key_cache.dtype
+    _check_i32(name, dev, page_table, query_starts, kv_lens)
+    seqs = kv_lens.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or query_starts.numel() != seqs + 1:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {seqs} sequences, a table of {tuple(page_table.shape)}, "
+                                         f"{query_starts.numel()} starts")
+    if q.dim() != 3 or q.dtype != dt:
+        raise CudaKernelError(ERR_TYPE, f"{name}: queries of {q.dtype} over a cache of {dt}")
+    rows, heads = q.shape[:2]
+    q = _rows3(name, q, dev, heads, dim)
+    if max_query_len < 0 or window < 0:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: max_query_len {max_query_len}, window {window}")
+    with _on_device(dev):
+        out, lse = _attention_out(name, q, out, out_dtype, return_lse)
+        nbytes = _attention_workspace(heads, kv_heads, dim)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        code = _lib.lib().hpc_paged_attention(
+            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), _DTYPE_IDS.get(dt, -1), pages, page_size,
+            page_table.data_ptr(), page_table.shape[1], query_starts.data_ptr(), kv_lens.data_ptr(), seqs, rows, heads,
+            kv_heads, dim, max_query_len, scale, window, ws.data_ptr(), nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype],
+            lse.data_ptr() if return_lse else None, _raw_stream(dev))
+    if code:
+        assert_cuda_ok(code, name)
+    return (out, lse) if return_lse else out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_starts: torch.Tensor, *,
+                     max_query_len: int, scale: float, window: int = 0, out: torch.Tensor | None = None,
+                     out_dtype: torch.dtype | None = None, return_lse: bool = False):
+    """Causal attention over whole prompts packed row behind row
+    (hpc_prompt_attention): q [rows][heads][head_dim], k and v
+    [rows][kv_heads][head_dim] (f16 or bf16; views with a row stride allowed),
+    sequence s = rows query_starts[s] .. query_starts[s+1]."""
+    name = "promptAttention"
+    dev, dt = q.device, q.dtype
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or not q.is_cuda:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: q, k and v are [rows][heads][head_dim] device tensors")
+    if k.dtype != dt or v.dtype != dt:
+        raise CudaKernelError(ERR_TYPE, f"{name}: queries of {dt}, keys of {k.dtype}, values of {v.dtype}")
+    rows, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape[0] != rows:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {rows} query rows, {k.shape[0]} key rows")
+    _check_i32(name, dev, query_starts)
+    seqs = query_starts.numel() - 1
+    if seqs < 0:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: query_starts is empty")
+    q, k, v = _rows3(name, q, dev, heads, dim), _rows3(name, k, dev, kv_heads, dim), _rows3(name, v, dev, kv_heads, dim)
+    if max_query_len < 0 or window < 0:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: max_query_len {max_query_len}, window {window}")
+    with _on_device(dev):
+        out, lse = _attention_out(name, q, out, out_dtype, return_lse)
+        nbytes = _attention_workspace(heads, kv_heads, dim)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        code = _lib.lib().hpc_prompt_attention(
+            q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _DTYPE_IDS.get(dt, -1),
+            query_starts.data_ptr(), seqs, rows, heads, kv_heads, dim, max_query_len, scale, window, ws.data_ptr(),
+            nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype], lse.data_ptr() if return_lse else None, _raw_stream(dev))
+    if code:
+        assert_cuda_ok(code, name)
+    return (out, lse) if return_lse else out

@@ -265,6 +265,82 @@ int hpc_lm_head_topk_noalloc(hpc_weight lm_head, const float *d_hidden, size_t h
                              size_t column_count, size_t k, int32_t id_offset, float softcap, int32_t *d_ids,
                              float *d_vals, void *stream);
 
+/* ---- serving many sequences: paged KV cache, attention, constrained top-k ----
+ * No reference counterpart (the reference decodes one sequence): the cache
+ * is cut into pages that sequences share out among themselves, a batch of
+ * sequences is packed row behind row, and one call serves all of them.
+ *
+ * Cache: keys and values [pages][page_size][kv_heads][head_dim], f16 or
+ * bf16; page_size a power of two from 16 to 1024, head_dim 64, 128 or 256,
+ * heads a multiple of kv_heads (query head h reads KV head
+ * h / (heads / kv_heads)).
+ * Batch: sequence s owns the packed rows query_starts[s] ..
+ * query_starts[s + 1] - 1 (its new tokens, in order); kv_lens[s] counts its
+ * tokens with the new ones, so row i stands at position kv_lens[s] - new + i;
+ * token j is in page page_table[s][j / page_size].  Rows behind
+ * query_starts[seqs] belong to no sequence: they are not read and their
+ * outputs are left as they were.  A row whose position is negative
+ * (kv_lens[s] below its new tokens) is not appended and sees no key.
+ * Lengths, starts and tables are read on the device, so captured graphs
+ * follow them.  A table entry outside the cache, a length beyond the table or
+ * starts outside the rows make the results of that call unspecified, touch
+ * no other memory, and are reported by the next hpc_device_error
+ * (HPC_ERR_SHAPE). */
+#define HPC_DTYPE_F32 0
+#define HPC_DTYPE_F16 1
+#define HPC_DTYPE_BF16 2
+
+/* Append: per new token and head, k = rope(rms(k) * k_norm) and v = rms(v)
+ * into the token's slot and q_out = rope(rms(q) * q_norm), in the order of
+ * the decode step (wasm/layers.ts:161-247).  Each part is optional: d_q_norm
+ * / d_k_norm NULL and norm_v 0 leave their norm out, rot_half 0 the
+ * rotation, d_q NULL the queries.  rms(x) = x / sqrt(mean(x^2) + eps); the
+ * rotation turns the pairs (i, i + rot_half), i < rot_half <= head_dim / 2, by
+ * position * inv_freq[i] radians (f64, reduced exactly; rot_half a multiple of
+ * head_dim / 32).  Inputs are f32 (what the matmuls here write) or the
+ * cache's type, [rows][heads][head_dim] with the given row strides in
+ * elements (views of one fused projection will do); q_out is contiguous, in
+ * the cache's type, and overlaps no input.  Sequences must not share the pages
+ * that they append to. */
+int hpc_paged_kv_append(const void *d_k, size_t k_stride, const void *d_v, size_t v_stride, const void *d_q,
+                        size_t q_stride, int in_dtype, size_t rows, size_t heads, size_t kv_heads, size_t head_dim,
+                        const double *d_inv_freq, size_t rot_half, const float *d_q_norm, const float *d_k_norm,
+                        int norm_v, double eps, void *d_key_cache, void *d_value_cache, int cache_dtype, size_t pages,
+                        size_t page_size, const int32_t *d_page_table, size_t table_width,
+                        const int32_t *d_query_starts, const int32_t *d_kv_lens, size_t seqs, void *d_q_out,
+                        void *stream);
+
+/* Workspace bytes of the two attention calls below, whatever the batch.  Calls
+ * that may overlap in time need a workspace each; nothing in it has to be
+ * kept or zeroed between calls. */
+int hpc_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t head_dim, size_t *out_bytes);
+
+/* Causal attention of every sequence's new rows over its pages:
+ * out = sum_j softmax_j(scale * q . k_j) v_j over the keys at positions
+ * <= the row's, and > the row's - window when window > 0.  q and the cache
+ * have one type; out is [rows][heads][head_dim] contiguous, of that type or
+ * f32; lse (optional, [rows][heads]) is the natural logarithm of the row's
+ * sum of exponentials.  A row that sees no key gets 0 and -inf.  Scores,
+ * maxima, sums and outputs are f32; probabilities are rounded to the cache's
+ * type before they multiply the values.  max_query_len: the most new tokens
+ * of any sequence (1 for a decode step); it chooses the kernel, not the
+ * result. */
+int hpc_paged_attention(const void *d_q, size_t q_stride, const void *d_key_cache, const void *d_value_cache,
+                        int cache_dtype, size_t pages, size_t page_size, const int32_t *d_page_table,
+                        size_t table_width, const int32_t *d_query_starts, const int32_t *d_kv_lens, size_t seqs,
+                        size_t rows, size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale,
+                        size_t window, void *d_workspace, size_t workspace_bytes, void *d_out, int out_dtype,
+                        float *d_lse, void *stream);
+
+/* The same over whole prompts that need no cache: keys and values are the
+ * packed rows themselves ([rows][kv_heads][head_dim], row strides in elements,
+ * multiples of 8), and every sequence attends within its own rows. */
+int hpc_prompt_attention(const void *d_q, size_t q_stride, const void *d_k, size_t k_stride, const void *d_v,
+                         size_t v_stride, int dtype, const int32_t *d_query_starts, size_t seqs, size_t rows,
+                         size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale,
+                         size_t window, void *d_workspace, size_t workspace_bytes, void *d_out, int out_dtype,
+                         float *d_lse, void *stream);
+
 /* ---- resident decoder model: decode / batched verify step ------------------
  * A Gemma-4-style decoder (pre/post RMSNorm sandwich, per-head QK norm, NeoX
  * RoPE, GQA over an fp32 KV cache, GEGLU FFN, tied Q6_K/Q4_K embedding / LM
