@@ -56,6 +56,9 @@ SIGNATURES = {
                                  C.c_float, _sz, _vp, _sz, _vp, _i, _vp, _vp]),
     "hpc_prompt_attention": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _i, _vp, _sz, _sz, _sz, _sz, _sz, _sz, C.c_float, _sz,
                                   _vp, _sz, _vp, _i, _vp, _vp]),
+    "hpc_logits_topk_workspace_bytes": (_i, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "hpc_logits_topk": (_i, [_vp, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz,
+                             _vp, _sz, _vp, _vp, _vp]),
     "hpc_model_create": (_i, [_vp, C.POINTER(_vp)]),
     "hpc_model_release": (_i, [_vp]),
     "hpc_model_set_weight": (_i, [_vp, _i, _i, _vp]),

@@ -552,3 +552,73 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_st
     if code:
         assert_cuda_ok(code, name)
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _logits_workspace(rows: int, vocab: int, k: int) -> int:
+    n = C.c_size_t()
+    assert_cuda_ok(_lib.lib().hpc_logits_topk_workspace_bytes(rows, vocab, k, C.byref(n)), "logitsTopK")
+    return n.value
+
+
+def logits_topk(logits: torch.Tensor, k: int, *, history: torch.Tensor | None = None,
+                history_starts: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                bias_values: torch.Tensor | None = None, bias_starts: torch.Tensor | None = None,
+                allowed: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Penalties for repeated tokens, biases and a grammar mask on logits
+    [rows][vocab] (f32), and the k best of every row (hpc_logits_topk): ids
+    (int32) and values, [rows][k], in the order sample_candidates takes;
+    (-1, -inf) where a row has fewer than k tokens left.
+
+    history: the rows' tokens one behind the other, row r's at
+    history_starts[r] .. [r+1], its first prompt_lens[r] of the prompt;
+    repetition, frequency, presence: one f32 per row; bias_ids / bias_values:
+    the same for biases with bias_starts; allowed: int32 words of 32 tokens,
+    [rows][>= ceil(vocab / 32)].  Logits and their history entries stay as
+    they are."""
+    name = "logitsTopK"
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+        raise CudaKernelError(ERR_TYPE, f"{name}: logits are [rows][vocab] float32 on a device")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if logits.stride(1) != 1 or logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    stride = logits.stride(0) if rows > 1 else max(vocab, 1)
+
+    def ptr(t, dtype, count, what):
+        if t is None:
+            return None
+        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (count is not None and t.numel() != count):
+            raise CudaKernelError(ERR_SHAPE, f"{name}: {what} is contiguous {dtype} on {dev}"
+                                             + ("" if count is None else f" with {count} values"))
+        return t.data_ptr() or None
+
+    if (history is None) != (history_starts is None):
+        raise CudaKernelError(ERR_ARG, f"{name}: history and history_starts go together")
+    if (bias_ids is None) != (bias_starts is None) or (bias_ids is None) != (bias_values is None):
+        raise CudaKernelError(ERR_ARG, f"{name}: bias_ids, bias_values and bias_starts go together")
+    i32, f32 = torch.int32, torch.float32
+    astride = 0
+    if allowed is not None:
+        if allowed.dim() != 2 or allowed.shape[0] != rows:
+            raise CudaKernelError(ERR_SHAPE, f"{name}: allowed is [rows][words]")
+        astride = allowed.shape[1]
+    hist_n = history.numel() if history is not None else 0
+    bias_n = bias_ids.numel() if bias_ids is not None else 0
+    args = (ptr(history, i32, None, "history"), hist_n, ptr(history_starts, i32, rows + 1, "history_starts"),
+            ptr(prompt_lens, i32, rows, "prompt_lens"), ptr(repetition, f32, rows, "repetition"),
+            ptr(frequency, f32, rows, "frequency"), ptr(presence, f32, rows, "presence"),
+            ptr(bias_ids, i32, None, "bias_ids"), ptr(bias_values, f32, bias_n, "bias_values"), bias_n,
+            ptr(bias_starts, i32, rows + 1, "bias_starts"), ptr(allowed, i32, None, "allowed"), astride)
+    nbytes = _logits_workspace(rows, vocab, k)
+    with _on_device(dev):
+        ids = torch.empty((rows, k), dtype=i32, device=dev)
+        vals = torch.empty((rows, k), dtype=f32, device=dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        code = _lib.lib().hpc_logits_topk(logits.data_ptr(), stride, rows, vocab, k, *args, ws.data_ptr(), nbytes,
+                                          ids.data_ptr(), vals.data_ptr(), _raw_stream(dev))
+    if code:
+        assert_cuda_ok(code, name)
+    return ids, vals

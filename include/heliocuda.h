@@ -341,6 +341,32 @@ int hpc_prompt_attention(const void *d_q, size_t q_stride, const void *d_k, size
                          size_t window, void *d_workspace, size_t workspace_bytes, void *d_out, int out_dtype,
                          float *d_lse, void *stream);
 
+/* Penalties, biases and a grammar mask on logits, and the k best (1..64, at
+ * most vocab) tokens of every row, in one pass over the logits.  Token i with
+ * logit l of a row, in f64 and rounded once to f32:
+ *   seen in the row's history:  x = l > 0 ? l / repetition : l * repetition
+ *   c > 0 times in its output:  x = x - frequency * c - presence
+ *   the row's biases of i, in list order:  x = x + bias
+ *   its mask bit is 0:          x = -inf
+ * History of row r: d_history[starts[r] .. starts[r + 1]), the first
+ * prompt_lens[r] entries its prompt (seen, not counted; NULL: none), the rest
+ * its output.  Ids outside the vocabulary are passed over; starts are bounded
+ * by history_len (bias_len).  Mask: bit i % 32 of word i / 32 of the row
+ * (allowed_stride words from row to row).  Every part is optional (NULL);
+ * repetition, frequency and presence are one f32 per row.
+ * ids / vals [rows][k]: value descending, then id ascending, as
+ * hpc_sample_candidates takes them.  A token whose value is -inf or NaN is
+ * never returned: a row with fewer than k others ends in (-1, -inf) entries.
+ * Softcapped logits are capped by the caller before. */
+#define HPC_LOGITS_MAX_VOCAB (1u << 20)
+int hpc_logits_topk_workspace_bytes(size_t rows, size_t vocab, size_t k, size_t *out_bytes);
+int hpc_logits_topk(const float *d_logits, size_t row_stride, size_t rows, size_t vocab, size_t k,
+                    const int32_t *d_history, size_t history_len, const int32_t *d_history_starts,
+                    const int32_t *d_prompt_lens, const float *d_repetition, const float *d_frequency,
+                    const float *d_presence, const int32_t *d_bias_ids, const float *d_bias_values, size_t bias_len,
+                    const int32_t *d_bias_starts, const uint32_t *d_allowed, size_t allowed_stride, void *d_workspace,
+                    size_t workspace_bytes, int32_t *d_ids, float *d_vals, void *stream);
+
 /* ---- resident decoder model: decode / batched verify step ------------------
  * A Gemma-4-style decoder (pre/post RMSNorm sandwich, per-head QK norm, NeoX
  * RoPE, GQA over an fp32 KV cache, GEGLU FFN, tied Q6_K/Q4_K embedding / LM
