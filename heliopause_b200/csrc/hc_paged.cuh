@@ -155,6 +155,9 @@ size_t attn_rows_workspace_bytes(int heads, int kv_heads, int dim);
 cudaError_t launch_attn_rows(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
                              cudaStream_t st);
 
+// Many query rows per sequence, on the tensor cores (hc_prompt_attn.cu).
+cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, cudaStream_t st);
+
 }  // namespace hc
 
 // Argument checks and the batch struct the paged entry points share

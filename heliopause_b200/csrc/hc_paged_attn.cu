@@ -808,7 +808,11 @@ int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSo
   a.out_f32 = out_dtype == HPC_DTYPE_F32;
   a.max_q = int(std::min(max_query_len, size_t(b.rows)));
   a.err = hc::device_status_word();
-  HPC_CK(hc::launch_attn_rows(a, b, kv, d_workspace, static_cast<cudaStream_t>(stream)), what);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Up to 64 rows (new tokens x heads of a group) the keys are read at most
+  // four times; beyond, a tensor-core tile of 128 rows pays.
+  const bool few = int64_t(a.max_q) * (a.heads / a.kv_heads) <= 64;
+  HPC_CK(few ? hc::launch_attn_rows(a, b, kv, d_workspace, st) : hc::launch_attn_prompt(a, b, kv, st), what);
   return HPC_OK;
 }
 
