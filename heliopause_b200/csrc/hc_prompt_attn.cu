@@ -48,7 +48,7 @@ template <int D>
 struct PrCfg {
   static constexpr int CG = D == 256 ? 2 : 1;             // CTAs per MMA
   static constexpr int NQ = D == 256 ? 1 : 2;             // row tiles per CTA
-  static constexpr int kThreads = 128 * NQ + 64;          // softmax warps, producer, MMA issuer
+  static constexpr int kThreads = 256 * NQ + 64;          // softmax warps, producer, MMA issuer
   static constexpr int kQ = PR_ROWS * D * 2;              // bytes of a row tile
   static constexpr int kK = PR_KEYS / CG * D * 2;         // bytes of K and V per stage in this CTA
   static constexpr int kStages = D == 64 ? 4 : 2;
@@ -138,6 +138,20 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {
       : PR_R8(r, 0), PR_R8(r, 8), PR_R8(r, 16), PR_R8(r, 24)
       : "r"(addr));
 }
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : PR_R8(r, 0), PR_R8(r, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      PR_I8(r, 0), PR_I8(r, 8)
+      : "memory");
+}
 __device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -181,7 +195,7 @@ __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
   } else {
     asm volatile(
         "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}\n" ::"r"(smem_u32(bar))
+        "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}\n" ::"r"(smem_u32(bar))
         : "memory");
   }
 }
@@ -194,23 +208,21 @@ __device__ __forceinline__ void sync_all() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
-// A bounded wait whose acquire reaches the other CTA of the pair.
-template <int CG>
-__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, int* err) {
-  if constexpr (CG == 1) return mbar_wait_parity(bar, parity, err);
+// mbar_wait_parity without a timer read where the phase is already complete.
+__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err) {
   unsigned long long t0 = 0;
   for (int it = 0;; ++it) {
     uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
     if (ok) return true;
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (it == 0) t0 = t;
-    else if (t - t0 > WAIT_LIMIT_NS) {
+    if (it == 0) {
+      t0 = t;
+    } else if (t - t0 > WAIT_LIMIT_NS) {
       if (err) atomicExch(err, DEVICE_ERR_TIMEOUT);
       return false;
     }
@@ -305,12 +317,13 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   __shared__ int s_item[3];  // sequence, KV head, tile
   __shared__ int s_sum[Cfg::kThreads / 32];
   __shared__ int s_odd;
+  __shared__ float s_half[2][2][NQ * PR_ROWS];  // [unit parity][column half][row]
   const int t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sq = base, sk = base + NQ * Cfg::kQ, sv = sk + ST * Cfg::kK;
   const int group = p.a.heads / p.a.kv_heads, window = p.a.window;
-  constexpr int PRODUCER = 4 * NQ, ISSUER = 4 * NQ + 1;
+  constexpr int PRODUCER = 8 * NQ, ISSUER = 8 * NQ + 1;
   if (warp == ISSUER) {
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     }
   }
   if (t == 0) {
-    mbar_init(&q_full, 4 * NQ * CG);
+    mbar_init(&q_full, 8 * NQ * CG);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -330,7 +343,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4 * CG);
+      mbar_init(&p_ready[i], 8 * CG);
       mbar_init(&pv_done[i], 1);
     }
     s_item[0] = -1;
@@ -408,7 +421,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         const int st = j % ST, ph = j / ST, k0 = (tile0 + j) * PR_KEYS;
         const int n = min(PR_KEYS, sp.len - k0);
         // K: this CTA's keys [k0 + rank * 128 / CG, ...), every piece
-        if (ph > 0) ok = wait_pair<CG>(&k_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
+        if (ph > 0) ok = pr_wait(&k_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const auto copies_k = [&](int r) {
@@ -428,7 +441,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
                      kv_head * Cfg::kPieces + piece, smem_u32(&k_full[st]) & (CG == 2 ? kLeaderMask : 0xffffffffu));
         }
         // V: every key, this CTA's pieces
-        if (ph > 0) ok = wait_pair<CG>(&v_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
+        if (ph > 0) ok = pr_wait(&v_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int cv = (n + p.box_v - 1) / p.box_v;
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         const int units = ntiles * NQ;
         const auto qk = [&](int u) {
           const int j = u / NQ, q = u % NQ, st = j % ST;
-          if (q == 0) ok = ok && wait_pair<CG>(&k_full[st], uint32_t(j / ST) & 1u, p.a.err);
+          if (q == 0) ok = ok && pr_wait(&k_full[st], uint32_t(j / ST) & 1u, p.a.err);
           if (!ok) return;
           tc_after();
 #pragma unroll
@@ -465,13 +478,13 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           pr_commit<CG>(&s_full[u & 1]);
           if (q == NQ - 1) pr_commit<CG>(&k_empty[st]);
         };
-        ok = wait_pair<CG>(&q_full, 0, p.a.err);
+        ok = pr_wait(&q_full, 0, p.a.err);
         qk(0);
         for (int u = 0; u < units && ok; ++u) {
           if (u + 1 < units) qk(u + 1);
           const int j = u / NQ, q = u % NQ, st = j % ST;
-          ok = ok && wait_pair<CG>(&p_ready[u & 1], uint32_t(u >> 1) & 1u, p.a.err);
-          ok = ok && wait_pair<CG>(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
+          ok = ok && pr_wait(&p_ready[u & 1], uint32_t(u >> 1) & 1u, p.a.err);
+          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
           if (!ok) break;
           tc_after();
 #pragma unroll
@@ -484,9 +497,10 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       }
       __syncwarp();
     } else {
-      // ---- softmax: thread = row of row tile q
-      const int q = warp >> 2, lt = t & 127;
+      // ---- softmax: thread = row of row tile q, half `half` of its columns
+      const int q = warp >> 3, half = (warp >> 2) & 1, lt = t & 127, lt2 = t & 255;
       const uint32_t lanes = uint32_t(warp & 3) * 32u << 16;
+      const int pair_bar = 1 + q * 4 + (warp & 3);  // the two warps that share 32 rows
       const int rt = r0 + (int(rank) * NQ + q) * PR_ROWS;  // the tile's first row
       const int r = rt + lt;
       const bool live = r < nrows;
@@ -500,7 +514,8 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       // lanes neighbouring bytes of a row.  A negative scale flips Q's sign.
       {
         const uint32_t flip = p.a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-        for (int i = lt; i < PR_ROWS * (D / 8); i += 128) {
+#pragma unroll 8
+        for (int i = lt2; i < PR_ROWS * (D / 8); i += 256) {
           const int rr = i / (D / 8), c = i % (D / 8), gr = rt + rr;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (gr < nrows && ntiles > 0) {
@@ -514,39 +529,45 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
                        : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive_leader<CG>(&q_full);
       }
+      constexpr int HC = PR_KEYS / 2;  // columns of a half
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < ntiles; ++j) {
         const int u = j * NQ + q, buf = u & 1, st = j % ST, k0 = (tile0 + j) * PR_KEYS;
-        ok = ok && wait_pair<CG>(&s_full[buf], uint32_t(u >> 1) & 1u, p.a.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        ok = ok && pr_wait(&s_full[buf], uint32_t(u >> 1) & 1u, p.a.err);
+        __syncwarp();
         tc_after();
-        uint32_t s[PR_KEYS];
+        uint32_t s[HC];
         const uint32_t sa = tmem + lanes + uint32_t(buf) * 128;
 #pragma unroll
-        for (int c = 0; c < PR_KEYS; c += 32) tm_ld32(sa + c, s + c);
+        for (int c = 0; c < HC; c += 32) tm_ld32(sa + half * HC + c, s + c);
         tm_wait_ld();
         const bool edge = k0 + PR_KEYS - 1 > all_hi || k0 < all_lo;
         if (edge) {
-          const int hi = lim - k0, lo = low - k0;
+          const int hi = lim - k0 - half * HC, lo = low - k0 - half * HC;
 #pragma unroll
-          for (int c = 0; c < PR_KEYS; ++c)
+          for (int c = 0; c < HC; ++c)
             if (c > hi || c < lo) s[c] = 0xff800000u;
         }
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
 #pragma unroll
-        for (int c = 4; c < PR_KEYS; c += 8)
+        for (int c = 4; c + 4 < HC; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            mx[e] = fmaxf(mx[e], __uint_as_float(s[c + e]));
-            if (c + 4 + e < PR_KEYS) mx[e] = fmaxf(mx[e], __uint_as_float(s[c + 4 + e]));
-          }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int e = 0; e < 4; ++e)
+            mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + e]), __uint_as_float(s[c + 4 + e])));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[HC - 4 + e]));
+        float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // the other half's maximum: one exchange between the two warps of the
+        // rows (the slot alternates, so the next one need not wait for readers)
+        s_half[j & 1][half][q * PR_ROWS + lt] = mt;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        mt = fmaxf(mt, s_half[j & 1][half ^ 1][q * PR_ROWS + lt]);
         const bool grew = mt > m && !((mt - m) * sc <= PR_GROW);  // m = -inf included
         if (__any_sync(0xffffffffu, grew)) {
           const float f = grew ? ex2((m - mt) * sc) : 1.0f;
@@ -554,40 +575,37 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           l *= f;
           if (j > 0) {
             const int up = u - NQ;  // the tile's previous product must have landed
-            ok = ok && wait_pair<CG>(&pv_done[up & 1], uint32_t(up >> 1) & 1u, p.a.err);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            ok = ok && pr_wait(&pv_done[up & 1], uint32_t(up >> 1) & 1u, p.a.err);
+            __syncwarp();
             tc_after();
-            const uint32_t oa = tmem + lanes + Cfg::kTmemO + uint32_t(q) * D;
+            const uint32_t oa = tmem + lanes + Cfg::kTmemO + uint32_t(q * D + half * (D / 2));
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tm_ld32(oa + c, o);
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              tm_ld16(oa + c, o);
               tm_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tm_st32(oa + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tm_st16(oa + c, o);
             }
-            tm_wait_st();
           }
         }
         const float ms = m == -INFINITY ? 0.0f : m * sc;
         const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(-ms, -ms);
         uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+        uint32_t pk[HC / 2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const uint64_t x = fma2(pack2(__uint_as_float(s[h * 64 + c]), __uint_as_float(s[h * 64 + c + 1])), sc2, nm2);
-            float a, b;
-            unpack2(x, a, b);
-            a = ex2(a), b = ex2(b);
-            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(a, b));
-            pk[c >> 1] = HalfOps<T>::pack(a, b);
-          }
-          tm_st32(sa + h * 32, pk);
+        for (int c = 0; c < HC; c += 2) {
+          const uint64_t x = fma2(pack2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nm2);
+          float a, b;
+          unpack2(x, a, b);
+          a = ex2(a), b = ex2(b);
+          sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(a, b));
+          pk[c >> 1] = HalfOps<T>::pack(a, b);
         }
+        // P takes the first half of S's columns: the other warp's scores are
+        // read (the exchange above came after both loads)
+        tm_st32(sa + half * (HC / 2), pk);
         {
           float a, b;
           unpack2(add2(sum[0], sum[1]), a, b);
@@ -595,22 +613,25 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         }
         if (edge) {
           // values of keys behind the end, and values that only some rows see
-          ok = ok && wait_pair<CG>(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
+          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
           ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
           const uint32_t vt = sv + st * Cfg::kK;
           bool odd = false;
-          for (int i = lt; i < PR_KEYS * Cfg::kPiecesV * 8; i += 128) {
-            const int key = i / (Cfg::kPiecesV * 8), c = i % (Cfg::kPiecesV * 8);
-            const uint32_t at = vt + (c >> 3) * (PR_KEYS * 128) + key * 128 + ((c & 7) << 4);
-            if (k0 + key >= sp.len) {
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-            } else {
-              uint32_t a, b, d, e;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(d), "=r"(e) : "r"(at) : "memory");
-              odd = odd || pr_not_finite<T>(a) || pr_not_finite<T>(b) || pr_not_finite<T>(d) || pr_not_finite<T>(e);
+          if (ok)
+            for (int i = lt2; i < PR_KEYS * Cfg::kPiecesV * 8; i += 256) {
+              const int key = i / (Cfg::kPiecesV * 8), c = i % (Cfg::kPiecesV * 8);
+              const uint32_t at = vt + (c >> 3) * (PR_KEYS * 128) + key * 128 + ((c & 7) << 4);
+              if (k0 + key >= sp.len) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+              } else {
+                uint32_t a, b, d, e;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(a), "=r"(b), "=r"(d), "=r"(e)
+                             : "r"(at)
+                             : "memory");
+                odd = odd || pr_not_finite<T>(a) || pr_not_finite<T>(b) || pr_not_finite<T>(d) || pr_not_finite<T>(e);
+              }
             }
-          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           if (__any_sync(0xffffffffu, odd) && lane == 0) {
             // both CTAs' rows are the sums of both CTAs' dims
@@ -625,25 +646,32 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
                     : "memory");
             }
           }
+          // what was written here is read by the pair's products
+          if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
         } else if (CG == 2) {
           // the issuer sees only its own CTA's V barrier: a CTA's arrival on
           // p_ready also says that its half of V has landed
-          ok = ok && wait_pair<CG>(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
+          __syncwarp();
         }
         tm_wait_st();
         tc_before();
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(&p_ready[buf]);
+        // a warp whose wait gave up walks on without arriving, to meet the
+        // other warp at the exchanges; nothing after it completes
+        ok = __all_sync(0xffffffffu, ok);
+        if (lane == 0 && ok) arrive_leader<CG>(&p_ready[buf]);
       }
       // ---- the rows' outputs
       if (ntiles > 0) {
         const int ul = (ntiles - 1) * NQ + q;
-        ok = ok && wait_pair<CG>(&pv_done[ul & 1], uint32_t(ul >> 1) & 1u, p.a.err);
+        ok = ok && pr_wait(&pv_done[ul & 1], uint32_t(ul >> 1) & 1u, p.a.err);
         ok = __all_sync(0xffffffffu, ok);
         tc_after();
       }
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");  // the last maxima are read
+      s_half[0][half][q * PR_ROWS + lt] = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      l = s_half[0][0][q * PR_ROWS + lt] + s_half[0][1][q * PR_ROWS + lt];
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
         const int64_t row = int64_t(sp.row0 + (live ? r : 0) / group) * p.a.heads + kv_head * group + (live ? r : 0) % group;
@@ -651,14 +679,14 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         float* out32 = p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr;
         float* lse = p.a.lse ? p.a.lse + row : nullptr;
         if (ntiles > 0 && *static_cast<volatile int*>(&s_odd)) {
-          if (live)
+          if (live && half == 0)
             pr_plain_row<T, D>(p, seq, sp.row0, kv_head,
                                static_cast<const T*>(p.a.q) + int64_t(sp.row0 + r / group) * p.a.q_stride +
                                    (kv_head * group + r % group) * D,
                                max(low, 0), lim, out, out32, lse);
         } else {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32];
             if (ntiles > 0) {
               tm_ld32(tmem + lanes + Cfg::kTmemO + uint32_t(q) * D + c, o);
@@ -686,14 +714,14 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
             }
             __syncwarp();
           }
-          if (live && lse) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
+          if (live && lse && half == 0) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
         }
       }
       // after a timeout the products in flight get one more bounded wait
       // before the tensor memory is freed
       if (!ok) {
-        wait_pair<CG>(&s_full[0], 0, nullptr);
-        wait_pair<CG>(&pv_done[0], 0, nullptr);
+        pr_wait(&s_full[0], 0, nullptr);
+        pr_wait(&pv_done[0], 0, nullptr);
       }
       __syncwarp();
     }
