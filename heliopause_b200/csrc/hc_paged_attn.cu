@@ -747,7 +747,7 @@ int hpc_paged_check(const char* what, size_t heads, size_t kv_heads, size_t head
     return hpc_fail(HPC_ERR_SHAPE, "%s: head_dim %zu (64, 128 or 256)", what, head_dim);
   if (kv_heads < 1 || heads < 1 || heads % kv_heads || heads > 1024)
     return hpc_fail(HPC_ERR_HEADS, "%s: %zu heads over %zu KV heads", what, heads, kv_heads);
-  if (rows > size_t(INT32_MAX) || seqs > (1u << 20))
+  if (rows > size_t(INT32_MAX) / heads || seqs > (1u << 20))
     return hpc_fail(HPC_ERR_SHAPE, "%s: %zu rows of %zu sequences", what, rows, seqs);
   if (page_size) {
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))

@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   __shared__ __align__(8) uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_ready[2], pv_done[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_item[3];  // sequence, KV head, tile
+  __shared__ SeqSpan s_span;
   __shared__ int s_sum[Cfg::kThreads / 32];
   __shared__ int s_odd;
   __shared__ float s_half[2][2][NQ * PR_ROWS];  // [unit parity][column half][row]
@@ -352,20 +353,22 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   pdl_wait_prior();
 
   // ---- which item: the sequences' tiles in order, each sequence's last rows
-  // (the longest sums) first, the KV heads of a tile side by side
+  // (the longest sums) first, the KV heads of a tile side by side.  Thread t
+  // counts sequences [t * per, ...); with up to one each, its span stays in
+  // registers and the lengths are read once.
   {
     const int x = int(blockIdx.x) / CG;
     const int per = (p.b.seqs + Cfg::kThreads - 1) / Cfg::kThreads;
-    const auto tiles = [&](int s, bool* bad) {
-      return (seq_span(p.b, s, bad).n * group + SPAN - 1) / SPAN * p.a.kv_heads;
-    };
+    const auto tiles = [&](const SeqSpan& q) { return (q.n * group + SPAN - 1) / SPAN * p.a.kv_heads; };
     int mine = 0;
+    SeqSpan own{};
     bool any_bad = false;
     for (int i = 0; i < per; ++i) {
       const int s = t * per + i;
       if (s >= p.b.seqs) break;
       bool bad;
-      mine += tiles(s, &bad);
+      own = seq_span(p.b, s, &bad);
+      mine += tiles(own);
       any_bad = any_bad || bad;
     }
     if (any_bad && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
@@ -383,11 +386,13 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       int at = incl - mine;
       for (int s = t * per;; ++s) {
         bool bad;
-        const int n = tiles(s, &bad);
+        const SeqSpan q = per == 1 ? own : seq_span(p.b, s, &bad);
+        const int n = tiles(q);
         if (x < at + n) {
           s_item[0] = s;
           s_item[1] = (x - at) % p.a.kv_heads;
           s_item[2] = n / p.a.kv_heads - 1 - (x - at) / p.a.kv_heads;
+          s_span = q;
           break;
         }
         at += n;
@@ -399,8 +404,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   const uint32_t tmem = s_tmem;
   const int seq = s_item[0], kv_head = s_item[1];
   if (seq >= 0) {
-    bool bad;
-    const SeqSpan sp = seq_span(p.b, seq, &bad);
+    const SeqSpan sp = s_span;
     const int nrows = sp.n * group, r0 = s_item[2] * SPAN, pos0 = sp.len - sp.n;
     const int p_first = pos0 + r0 / group, p_last = pos0 + (min(r0 + SPAN, nrows) - 1) / group;
     const int key_lo = window > 0 ? max(0, p_first - window + 1) : 0, key_hi = min(sp.len, p_last + 1);
@@ -510,23 +514,42 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       const int all_hi = min(sp.len - 1, pos0 + min(rt, nrows - 1) / group);
       const int all_lo = window > 0 ? pos0 + min(rt + PR_ROWS - 1, nrows - 1) / group - window + 1 : 0;
       const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
-      // Q into the swizzled operand layout; 16 bytes at a time, neighbouring
-      // lanes neighbouring bytes of a row.  A negative scale flips Q's sign.
+      // Rows of the tile to (token, head of the group): row rr is pair
+      // rem + rr counted from token tok0, divided by a multiplication (exact
+      // below 2^21 / group, and rem + rr < 1152)
+      const int tok0 = rt / group, rem = rt - tok0 * group;
+      const uint32_t inv_group = ((1u << 21) + uint32_t(group) - 1u) / uint32_t(group);
+      const auto row_at = [&](int rr) {  // element offset of the row's head in a [row][heads][D] tensor, less the token's
+        const int x = rem + rr, tok = int((uint32_t(x) * inv_group) >> 21);
+        return make_int2(sp.row0 + tok0 + tok, kv_head * group + x - tok * group);
+      };
+      // Q into the swizzled operand layout, 16 bytes at a time, neighbouring
+      // lanes neighbouring bytes of a row, eight loads in flight per thread.
+      // A negative scale flips Q's sign.
       {
         const uint32_t flip = p.a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 8
-        for (int i = lt2; i < PR_ROWS * (D / 8); i += 256) {
-          const int rr = i / (D / 8), c = i % (D / 8), gr = rt + rr;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (gr < nrows && ntiles > 0) {
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + int64_t(sp.row0 + gr / group) * p.a.q_stride +
-                                                (kv_head * group + gr % group) * D + c * 8);
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        constexpr int N = PR_ROWS * (D / 8) / 256, B = N < 8 ? N : 8;
+#pragma unroll 1
+        for (int i0 = 0; i0 < N; i0 += B) {
+          uint4 v[B];
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const int at = (i0 + i) * 256 + lt2, rr = at / (D / 8), c = at % (D / 8);
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (rt + rr < nrows && ntiles > 0) {
+              const int2 w = row_at(rr);
+              v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + int64_t(w.x) * p.a.q_stride + w.y * D +
+                                                     c * 8);
+            }
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + q * Cfg::kQ + (c >> 3) * (PR_ROWS * 128) +
-                                                                       rr * 128 + (((c & 7) ^ (rr & 7)) << 4)),
-                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                       : "memory");
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const int at = (i0 + i) * 256 + lt2, rr = at / (D / 8), c = at % (D / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + q * Cfg::kQ + (c >> 3) * (PR_ROWS * 128) +
+                                                                         rr * 128 + (((c & 7) ^ (rr & 7)) << 4)),
+                         "r"(v[i].x ^ flip), "r"(v[i].y ^ flip), "r"(v[i].z ^ flip), "r"(v[i].w ^ flip)
+                         : "memory");
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
@@ -674,17 +697,19 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       l = s_half[0][0][q * PR_ROWS + lt] + s_half[0][1][q * PR_ROWS + lt];
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-        const int64_t row = int64_t(sp.row0 + (live ? r : 0) / group) * p.a.heads + kv_head * group + (live ? r : 0) % group;
-        T* out = static_cast<T*>(p.a.out) + row * D;
-        float* out32 = p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr;
+        const int2 own = row_at(live ? lt : 0);
+        const int64_t row = int64_t(own.x) * p.a.heads + own.y;
         float* lse = p.a.lse ? p.a.lse + row : nullptr;
         if (ntiles > 0 && *static_cast<volatile int*>(&s_odd)) {
           if (live && half == 0)
-            pr_plain_row<T, D>(p, seq, sp.row0, kv_head,
-                               static_cast<const T*>(p.a.q) + int64_t(sp.row0 + r / group) * p.a.q_stride +
-                                   (kv_head * group + r % group) * D,
-                               max(low, 0), lim, out, out32, lse);
+            pr_plain_row<T, D>(p, seq, sp.row0, kv_head, static_cast<const T*>(p.a.q) + int64_t(own.x) * p.a.q_stride + own.y * D,
+                               max(low, 0), lim, static_cast<T*>(p.a.out) + row * D,
+                               p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr, lse);
         } else {
+          // through shared memory (the operands are done with), so that a warp
+          // stores whole rows: 16-byte chunk c of row rr at chunk c ^ (rr % 8)
+          const int chunks = p.a.out_f32 ? D / 4 : D / 8;  // 16-byte chunks of a row
+          const uint32_t stage = base + uint32_t(q * PR_ROWS) * chunks * 16;
 #pragma unroll 1
           for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32];
@@ -695,26 +720,46 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = 0;
             }
-            if (!live) {
-            } else if (out32) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(out32 + c + e) =
-                    make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+            const auto put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (lt * chunks + (chunk ^ (lt & 7))) * 16), "r"(x),
+                           "r"(y), "r"(z), "r"(w)
+                           : "memory");
+            };
+            if (p.a.out_f32) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) put((c + e) / 4, o[e], o[e + 1], o[e + 2], o[e + 3]);
             } else {
+              uint32_t w[16];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint32_t w[4];
+              for (int e = 0; e < 16; ++e)
+                w[e] = HalfOps<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w[i] = HalfOps<T>::pack(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
-                *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+              for (int e = 0; e < 16; e += 4) put((c + 2 * e) / 8, w[e], w[e + 1], w[e + 2], w[e + 3]);
             }
-            __syncwarp();
           }
           if (live && lse && half == 0) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
+        }
+      }
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      if (ok && !(ntiles > 0 && *static_cast<volatile int*>(&s_odd))) {
+        // the two warps of these 32 rows store 16 rows each
+        const int chunks = p.a.out_f32 ? D / 4 : D / 8;
+        const uint32_t stage = base + uint32_t(q * PR_ROWS) * chunks * 16;
+        const int first = (warp & 3) * 32 + half * 16;
+        const int shift = 31 - __clz(chunks);
+#pragma unroll 4
+        for (int i = lane; i < 16 * chunks; i += 32) {
+          const int rr = first + (i >> shift), c = i & (chunks - 1);
+          if (rt + rr >= nrows) break;
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + (rr * chunks + (c ^ (rr & 7))) * 16)
+                       : "memory");
+          const int2 w = row_at(rr);
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.a.out) + ((int64_t(w.x) * p.a.heads + w.y) * chunks + c) * 16) = v;
         }
       }
       // after a timeout the products in flight get one more bounded wait
