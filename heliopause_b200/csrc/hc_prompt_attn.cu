@@ -2,62 +2,79 @@
 // chunks of them, on the fifth-generation tensor cores.
 //
 // The rows of one product are (new token, query head of the KV head's group)
-// pairs in token order, 128 to a tile, so a tile covers 128 / group tokens: a
+// pairs in token order, 128 to a CTA, so a tile covers 128 / group tokens: a
 // short prompt still fills tiles, a tile's causal border is narrow, and a key
 // tile read once serves the whole group.  Per tile of 128 keys:
 //   S = Q K^T      tcgen05.mma, both operands in shared memory, S f32 in
-//                  tensor memory (128 columns, two buffers);
+//                  tensor memory;
 //   P = 2^(S c - m c), c = scale log2(e): one thread per row, so maximum and
-//                  sum (f32, of the unrounded P) need no exchange; P is rounded to
-//                  the value type and replaces S in tensor memory;
+//                  sum (f32, of the unrounded P) stay in registers; P is rounded
+//                  to the value type and goes to tensor memory;
 //   O += P V       tcgen05.mma with P read from tensor memory, O f32 there
-//                  (dim columns).
+//                  (head_dim columns).
 // m is the row's running maximum, but moved only when it grew by more than 8
 // (in log2 units): P then stays below 2^8, which no type here minds, and the pass
 // over O in tensor memory that a new maximum needs becomes rare (the first
-// few tiles).  The tensor core runs S of unit u + 1 before O of unit u, so the
-// exponentials of one unit hide behind the products of another.
+// few tiles).
 //
-// head_dim 64 and 128: one CTA, two row tiles (256 rows) that take turns: per
-//   key tile 4 products, each K and V byte is used by 256 rows.
-// head_dim 256: O alone takes 256 of the 512 columns, so a CTA holds one row tile and
-//   two CTAs form a pair (cta_group::2): M = 256, each CTA brings half of the
-//   keys of K and half of the dims of V, so again each byte serves 256 rows --
-//   with one tile per CTA the K and V traffic from L2 would be 64 bytes per clock
-//   and SM, which it does not deliver -- and shared memory holds two stages of each.
+// head_dim 128 and 256: two CTAs form a pair (cta_group::2, M = 256), each bringing
+//   its 128 rows, half of the keys of K and half of the dims of V.  One CTA's
+//   products of N = 128 read 128 bytes of shared memory per clock, all that there
+//   is, and the arriving tiles come on top; in a pair the second operand is
+//   shared, and K and V cross from L2 once for 256 rows.
+// head_dim 64: one CTA; the exponentials bound it, not the products.
+//
+// Two warpgroups take the key tiles in turn, so that one's loads, maxima and
+// barriers fall into the other's exponentials; they pass the row's m
+// along in shared memory.  Tensor memory: O behind column 256, two S slots of 128
+// columns; up to head_dim 128 P has two slots of 64 of its own, so an S slot is
+// free as soon as its row is in registers and the next S does not wait for P.
+// At head_dim 256 P takes the place of its S.
+//
+// The CTAs stay: each takes its next item (sequence, KV head, rows) from the
+// launch by clusterlaunchcontrol while it works on the present one, the
+// longest sums first, and loads its Q, K and V ahead, so that only the rows'
+// store falls between two items.
 //
 // K and V arrive by TMA, page by page or straight from packed rows, 128-byte
 // swizzled, which is the operand layout of both products (K rows are K-major; V is
 // N-major as it lies).  Keys that a row does not see get -inf scores and add
-// nothing: values behind the sequence's end are zeroed before they are
+// nothing: values behind the last key in use are zeroed before they are
 // multiplied, and if a value that only some rows of a tile see is not finite
 // (0 * inf), the tile's rows are summed again by plain loops over what they see.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "hc_paged.cuh"
 
 namespace hc {
 namespace {
 
-constexpr int PR_KEYS = 128;  // keys per tile
-constexpr int PR_ROWS = 128;  // rows per tile
+constexpr int PR_KEYS = 128;     // keys per tile
+constexpr int PR_ROWS = 128;     // rows per CTA
 constexpr float PR_GROW = 8.0f;  // log2 units a maximum may grow before O is rescaled
 
 template <int D>
 struct PrCfg {
-  static constexpr int CG = D == 256 ? 2 : 1;             // CTAs per MMA
-  static constexpr int NQ = D == 256 ? 1 : 2;             // row tiles per CTA
-  static constexpr int kThreads = 256 * NQ + 64;          // softmax warps, producer, MMA issuer
-  static constexpr int kQ = PR_ROWS * D * 2;              // bytes of a row tile
-  static constexpr int kK = PR_KEYS / CG * D * 2;         // bytes of K and V per stage in this CTA
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kSmem = 1024 + NQ * kQ + 2 * kStages * kK;
-  static constexpr int kBoxK = PR_KEYS / CG;              // most key rows per TMA copy of K
+  static constexpr int CG = D == 64 ? 1 : 2;              // CTAs per MMA
+  static constexpr bool kOwnP = D <= 128;                 // P beside S, not over it
+  static constexpr uint32_t kTmemO = D == 256 ? 256 : 384;
+  static constexpr int kThreads = 384;                    // 8 softmax warps, producer, issuer, 2 loaders
+  static constexpr int kQ = PR_ROWS * D * 2;              // bytes of Q
+  static constexpr int kK = PR_KEYS / CG * D * 2;         // bytes of K and of V per stage in this CTA
+  static constexpr int kStages = D == 256 ? 2 : 4;
+  static constexpr int kStage = 8 * 32 * 64;              // output staging: 32 rows x 64 bytes per warp
+  static constexpr int kSmem = 1024 + kQ + 2 * kStages * kK + kStage;
+  static constexpr int kKeys = PR_KEYS / CG;              // keys of K in this CTA
   static constexpr int kPieces = D / 64;                  // 128-byte pieces of a row
   static constexpr int kPiecesV = kPieces / CG;           // of them V pieces in this CTA
-  static constexpr uint32_t kTmemO = 256;                 // column of O (S buffers at 0 and 128)
+  __host__ __device__ static constexpr uint32_t p_col(uint32_t slot) { return kOwnP ? 256 + slot * 64 : slot * 128; }
 };
+// registers per thread: launched with 168, the two softmax warpgroups take 208
+// (a row of 128 scores each) from the third
+constexpr int PR_REGS_SOFTMAX = 208, PR_REGS_OTHER = 88;
+static_assert(2 * PR_REGS_SOFTMAX + PR_REGS_OTHER == 3 * 168, "the split is of what the block was launched with");
 
 struct PrArgs {
   AttnArgs a;
@@ -65,7 +82,7 @@ struct PrArgs {
   const void* k;       // for the plain loops
   const void* v;
   int64_t k_stride, v_stride;
-  int box_k, box_v;    // key rows per TMA copy
+  int box_k, box_v;    // key rows per TMA copy, as powers of two
   int64_t slots;
 };
 
@@ -152,13 +169,6 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
       PR_I8(r, 0), PR_I8(r, 8)
       : "memory");
 }
-__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      PR_I8(r, 0), PR_I8(r, 8), PR_I8(r, 16), PR_I8(r, 24)
-      : "memory");
-}
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -179,6 +189,39 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// The larger of three; NaN if one is NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x for a pair on the FMA pipe: x = n + f with n the nearest integer (in the
+// low bits after adding 1.5 * 2^23), a polynomial of degree 4 for 2^f on
+// [-1/2, 1/2] (the minimax one for the relative error, 2.6e-6, by Remez
+// exchange), and n added to the exponent.  x is at most 8 here and
+// taken as -126 where it is less.  The special-function unit delivers 16
+// results per clock and SM, one tile's exponentials take as long as a
+// head_dim 128 tile's products; every PR_POLY_EVERY-th pair goes this way.
+constexpr int PR_POLY_EVERY = 1000;
+__device__ __forceinline__ void ex2_poly2(uint64_t x, float& e0, float& e1) {
+  float a, b;
+  unpack2(x, a, b);
+  const uint64_t y = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t t = add2(y, pack2(12582912.0f, 12582912.0f));
+  const uint64_t n = add2(t, pack2(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), y);
+  uint64_t q = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
+  q = fma2(q, f, pack2(0.240247443318367f, 0.240247443318367f));
+  q = fma2(q, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  unpack2(t, t0, t1);
+  unpack2(q, e0, e1);
+  e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(t0) << 23));
+  e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(t1) << 23));
 }
 
 // ---- barriers across a CTA pair -------------------------------------------------
@@ -208,16 +251,19 @@ __device__ __forceinline__ void sync_all() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
+__device__ __forceinline__ bool pr_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
 // mbar_wait_parity without a timer read where the phase is already complete.
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err) {
   unsigned long long t0 = 0;
   for (int it = 0;; ++it) {
-    uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(parity)
-                 : "memory");
-    if (ok) return true;
+    if (pr_try(bar, parity)) return true;
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     if (it == 0) {
@@ -227,6 +273,54 @@ __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err
       return false;
     }
   }
+}
+// Two barriers with their answers in flight together: the common case, both
+// complete, costs one round trip instead of two.
+__device__ __forceinline__ bool pr_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* err) {
+  const bool x = pr_try(a, pa), y = pr_try(b, pb);
+  return (x || pr_wait(a, pa, err)) && (y || pr_wait(b, pb, err));
+}
+
+// One lane of the converged warp.  The issuer's loop runs in the whole warp, on
+// values that are the same in every lane, and only the instructions that one
+// thread has to issue stand behind this: inside a branch on the lane number
+// the compiler passes each MMA's operands one by one (about 80 clocks per MMA).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
+}
+
+// ---- the launch's next item (clusterlaunchcontrol) ------------------------------
+
+// Asks for a cluster of this grid that has not started; the answer (16 bytes)
+// arrives on `bar` in every CTA of the cluster.
+template <int CG>
+__device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
+  if constexpr (CG == 1)
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+  else
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.multicast::cluster::all.b128 "
+        "[%0], [%1];" ::"r"(smem_u32(answer)),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+// The first block of the cluster taken over, or -1 when none is left.
+__device__ __forceinline__ int clc_answer(const uint4* answer) {
+  uint32_t x, got;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z;\n\tld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %1, 1, 0, p;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, _}, r;\n\t}\n"
+      : "=&r"(x), "=&r"(got)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got ? int(x) : -1;
 }
 
 template <int CG>
@@ -304,27 +398,56 @@ __device__ __forceinline__ bool pr_not_finite(uint32_t v) {
 
 // ---- the kernel ---------------------------------------------------------------------
 
+// An item as the scheduler hands it out; seq < 0: there is none left.
+struct PrItem {
+  int seq, head, tile;
+  SeqSpan span;
+};
+
+// What every role derives from an item.
+struct PrGeom {
+  int nrows, r0, pos0;  // rows of the sequence's product, the item's first, position of the first new token
+  int key0, key_hi;     // first key of the first tile, one behind the last key that a row sees
+  int units;            // key tiles
+};
+__device__ __forceinline__ PrGeom pr_geom(const PrItem& it, int group, int window, int rows_per_item) {
+  PrGeom g;
+  g.nrows = it.span.n * group;
+  g.r0 = it.tile * rows_per_item;
+  g.pos0 = it.span.len - it.span.n;
+  const int p_first = g.pos0 + g.r0 / group, p_last = g.pos0 + (min(g.r0 + rows_per_item, g.nrows) - 1) / group;
+  const int key_lo = window > 0 ? max(0, p_first - window + 1) : 0;
+  g.key_hi = min(it.span.len, p_last + 1);
+  g.key0 = key_lo / PR_KEYS * PR_KEYS;
+  g.units = g.key_hi > key_lo ? (g.key_hi - g.key0 + PR_KEYS - 1) / PR_KEYS : 0;
+  return g;
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     hc_prompt_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                           const __grid_constant__ PrArgs p) {
   using Cfg = PrCfg<D>;
-  constexpr int CG = Cfg::CG, NQ = Cfg::NQ, ST = Cfg::kStages, SPAN = PR_ROWS * NQ * CG;
+  constexpr int CG = Cfg::CG, ST = Cfg::kStages, SPAN = PR_ROWS * CG;
   constexpr uint32_t FMT = HalfOps<T>::kMap == CU_TENSOR_MAP_DATA_TYPE_FLOAT16 ? 0u : 1u;
+  constexpr int PRODUCER = 8, ISSUER = 9, SCHEDULER = 10, ISSUER_O = 11;  // (11: a second loader at head_dim 256)
+  constexpr int LOADERS = Cfg::kOwnP ? 1 : 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_ready[2], pv_done[2];
+  __shared__ __align__(16) uint4 clc_resp;
+  __shared__ __align__(8) uint64_t q_first, q_full, q_free, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], v_peer[ST];
+  __shared__ __align__(8) uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free, m_pass[4], l_pass[4];
+  __shared__ __align__(8) uint64_t item_full[2], item_empty[2], clc_full, clc_ready;
+  __shared__ PrItem s_items[2];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_item[3];  // sequence, KV head, tile
-  __shared__ SeqSpan s_span;
-  __shared__ int s_sum[Cfg::kThreads / 32];
-  __shared__ int s_odd;
-  __shared__ float s_half[2][2][NQ * PR_ROWS];  // [unit parity][column half][row]
+  __shared__ int s_odd[4];              // item number + 1 of a tile with a value that is not finite
+  __shared__ float s_m[PR_ROWS];        // the rows' m after the last tile decided
+  __shared__ float2 s_l[2][2][PR_ROWS]; // [item parity] (m, l) of each warpgroup at an item's end
   const int t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sq = base, sk = base + NQ * Cfg::kQ, sv = sk + ST * Cfg::kK;
+  const uint32_t sq = base, sk = base + Cfg::kQ, sv = sk + ST * Cfg::kK, so = sv + ST * Cfg::kK;
   const int group = p.a.heads / p.a.kv_heads, window = p.a.window;
-  constexpr int PRODUCER = 8 * NQ, ISSUER = 8 * NQ + 1;
+  int* const err = p.a.err;
   if (warp == ISSUER) {
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
@@ -335,316 +458,510 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     }
   }
   if (t == 0) {
-    mbar_init(&q_full, 8 * NQ * CG);
+    mbar_init(&q_first, 8 * CG);
+    mbar_init(&q_full, LOADERS * CG);
+    mbar_init(&q_free, 1);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_peer[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 8 * CG);
+      mbar_init(&s_free[i], 4 * CG);
+      mbar_init(&p_ready[i], 4 * CG);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);  // every warp but the scheduler
     }
-    s_item[0] = -1;
-    s_odd = 0;
+    for (int w = 0; w < 4; ++w) {
+      mbar_init(&m_pass[w], 1);
+      mbar_init(&l_pass[w], 2);
+    }
+    mbar_init(&o_free, 8 * CG);
+    mbar_init(&clc_full, 1);
+    mbar_init(&clc_ready, 1);
+    for (int i = 0; i < 4; ++i) s_odd[i] = 0;
   }
-  pdl_wait_prior();
-
-  // ---- which item: the sequences' tiles in order, each sequence's last rows
-  // (the longest sums) first, the KV heads of a tile side by side.  Thread t
-  // counts sequences [t * per, ...); with up to one each, its span stays in
-  // registers and the lengths are read once.
-  {
-    const int x = int(blockIdx.x) / CG;
-    const int per = (p.b.seqs + Cfg::kThreads - 1) / Cfg::kThreads;
-    const auto tiles = [&](const SeqSpan& q) { return (q.n * group + SPAN - 1) / SPAN * p.a.kv_heads; };
-    int mine = 0;
-    SeqSpan own{};
-    bool any_bad = false;
-    for (int i = 0; i < per; ++i) {
-      const int s = t * per + i;
-      if (s >= p.b.seqs) break;
-      bool bad;
-      own = seq_span(p.b, s, &bad);
-      mine += tiles(own);
-      any_bad = any_bad || bad;
-    }
-    if (any_bad && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_sum[warp] = incl;
-    tc_before();
-    __syncthreads();
-    for (int i = 0; i < warp; ++i) incl += s_sum[i];
-    if (incl - mine <= x && x < incl) {
-      int at = incl - mine;
-      for (int s = t * per;; ++s) {
-        bool bad;
-        const SeqSpan q = per == 1 ? own : seq_span(p.b, s, &bad);
-        const int n = tiles(q);
-        if (x < at + n) {
-          s_item[0] = s;
-          s_item[1] = (x - at) % p.a.kv_heads;
-          s_item[2] = n / p.a.kv_heads - 1 - (x - at) / p.a.kv_heads;
-          s_span = q;
-          break;
-        }
-        at += n;
-      }
-    }
-  }
+  tc_before();
   sync_all<CG>();
   tc_after();
   const uint32_t tmem = s_tmem;
-  const int seq = s_item[0], kv_head = s_item[1];
-  if (seq >= 0) {
-    const SeqSpan sp = s_span;
-    const int nrows = sp.n * group, r0 = s_item[2] * SPAN, pos0 = sp.len - sp.n;
-    const int p_first = pos0 + r0 / group, p_last = pos0 + (min(r0 + SPAN, nrows) - 1) / group;
-    const int key_lo = window > 0 ? max(0, p_first - window + 1) : 0, key_hi = min(sp.len, p_last + 1);
-    const int tile0 = key_lo / PR_KEYS;
-    const int ntiles = key_hi > key_lo ? (key_hi + PR_KEYS - 1) / PR_KEYS - tile0 : 0;
-    bool ok = true;
+  pdl_wait_prior();
+  bool ok = true;
 
-    if (warp == PRODUCER) {
-      // ---- K and V tiles; lane i takes copies i, i + 32, ... of (page, piece)
+  // Item i of this CTA, read by every warp from the ring.
+  const auto next_item = [&](int i, PrItem* it) {
+    ok = ok && pr_wait(&item_full[i & 1], uint32_t(i >> 1) & 1u, err);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return false;
+    *it = s_items[i & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+    return it->seq >= 0;
+  };
+  // Rows of the CTA's tile: row rr is pair rem + rr counted from token tok0,
+  // divided by a multiplication (exact for rem + rr < 2^21 / group; it is below
+  // 1152).
+  const uint32_t inv_group = ((1u << 21) + uint32_t(group) - 1u) / uint32_t(group);
+  const auto row_at = [&](int tok0, int rem, int rr) {  // (token, head of the group)
+    const int x = rem + rr, tok = int((uint32_t(x) * inv_group) >> 21);
+    return make_int2(tok0 + tok, x - tok * group);
+  };
+  // The CTA's rows of an item into the swizzled operand layout by `n` threads: 16
+  // bytes at a time, neighbouring lanes neighbouring bytes of a row, all copies
+  // in flight together.  A negative scale flips Q's sign (so that the maximum
+  // is that of the scores).
+  const auto load_q = [&](const PrItem& it, const PrGeom& g, int i0, int n) {
+    const int rt = g.r0 + int(rank) * PR_ROWS;
+    const int tok0 = rt / group, rem = rt - tok0 * group;
+    const T* src = static_cast<const T*>(p.a.q) + int64_t(it.span.row0) * p.a.q_stride + it.head * group * D;
+    const auto dst = [&](int i) {
+      const int rr = i / (D / 8), c = i % (D / 8);
+      return sq + (c >> 3) * (PR_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+    };
+#pragma unroll 4
+    for (int i = i0; i < PR_ROWS * (D / 8); i += n) {
+      const int rr = i / (D / 8), c = i % (D / 8);
+      const bool in = rt + rr < g.nrows;
+      const int2 w = row_at(tok0, rem, in ? rr : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst(i)),
+                   "l"(in ? src + int64_t(w.x) * p.a.q_stride + w.y * D + c * 8 : src), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+    cp_async_wait_all();
+    if (p.a.scale_log2 < 0.0f)
+      for (int i = i0; i < PR_ROWS * (D / 8); i += n) {
+        uint32_t x, y, z, w;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(dst(i)) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst(i)), "r"(x ^ 0x80008000u), "r"(y ^ 0x80008000u),
+                     "r"(z ^ 0x80008000u), "r"(w ^ 0x80008000u)
+                     : "memory");
+      }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    __syncwarp();
+  };
+
+  if (warp >= PRODUCER) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
+  if (warp == PRODUCER) {
+    // ---- K and V tiles, K one ahead of V (its product comes first).  Lane i
+    // looks up the tile's i-th page; one lane issues the copies, with operands
+    // that are uniform in the warp (see elect_one: from a lane each they took
+    // 1900 clocks a tile)
+    PrItem it;
+    const int bk = 1 << p.box_k, bv = 1 << p.box_v;  // (divisions here would cost as much as a tile's products)
+    int k_st = 0, v_st = 0;
+    uint32_t k_ph = 1, v_ph = 1;  // parity of the stage's last release; the first use waits for none
+    for (int n_it = 0; next_item(n_it, &it); ++n_it) {
+      const PrGeom g = pr_geom(it, group, window, SPAN);
       const auto row_of = [&](int key) {
-        if (!p.b.table) return sp.row0 + key;
-        const int page = p.b.table[int64_t(seq) * p.b.width + (key >> p.b.page_shift)];
+        if (!p.b.table) return it.span.row0 + key;
+        const int page = p.b.table[int64_t(it.seq) * p.b.width + (key >> p.b.page_shift)];
         const bool in = page >= 0 && page < p.b.pages;
-        if (!in && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
+        if (!in && err) atomicExch(err, DEVICE_ERR_PAGE);
         return in ? int((int64_t(page) << p.b.page_shift) + (key & ((1 << p.b.page_shift) - 1))) : int(p.slots);
       };
-      for (int j = 0; j < ntiles && ok; ++j) {
-        const int st = j % ST, ph = j / ST, k0 = (tile0 + j) * PR_KEYS;
-        const int n = min(PR_KEYS, sp.len - k0);
-        // K: this CTA's keys [k0 + rank * 128 / CG, ...), every piece
-        if (ph > 0) ok = pr_wait(&k_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const auto copies_k = [&](int r) {
-          return (min(Cfg::kBoxK, max(0, n - r * Cfg::kBoxK)) + p.box_k - 1) / p.box_k;
-        };
-        if (lane == 0 && rank == 0) {
-          int c = 0;
-          for (int r = 0; r < CG; ++r) c += copies_k(r);
-          mbar_expect_tx(&k_full[st], uint32_t(c * p.box_k * D * 2));
+      for (int i = 0; i <= g.units && ok && g.units > 0; ++i) {
+        if (i < g.units) {  // K: this CTA's keys, every piece
+          const int k0 = g.key0 + i * PR_KEYS, n = min(PR_KEYS, g.key_hi - k0);
+          ok = pr_wait(&k_empty[k_st], k_ph, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const auto copies = [&](int r) { return (min(Cfg::kKeys, max(0, n - r * Cfg::kKeys)) + bk - 1) >> p.box_k; };
+          if (rank == 0 && elect_one()) {
+            int c = copies(0);
+            if (CG == 2) c += copies(1);
+            mbar_expect_tx(&k_full[k_st], uint32_t(c * bk * D * 2));
+          }
+          __syncwarp();
+          const int c_n = copies(int(rank));
+          const int row = lane < c_n ? row_of(k0 + int(rank) * Cfg::kKeys + lane * bk) : 0;
+          const uint32_t bar = smem_u32(&k_full[k_st]) & (CG == 2 ? kLeaderMask : 0xffffffffu);
+          for (int c = 0; c < c_n; ++c) {
+            const int r = __shfl_sync(0xffffffffu, row, c);
+            if (elect_one()) {
+#pragma unroll
+              for (int piece = 0; piece < Cfg::kPieces; ++piece)
+                pr_tma<CG>(sk + k_st * Cfg::kK + piece * (Cfg::kKeys * 128) + c * bk * 128, &kmap, r,
+                           it.head * Cfg::kPieces + piece, bar);
+            }
+            __syncwarp();
+          }
+          if (++k_st == ST) k_st = 0, k_ph ^= 1u;
         }
-        __syncwarp();
-        const int ck = copies_k(int(rank));
-        for (int i = lane; i < ck * Cfg::kPieces; i += 32) {
-          const int c = i / Cfg::kPieces, piece = i % Cfg::kPieces;
-          const int row = row_of(k0 + int(rank) * Cfg::kBoxK + c * p.box_k);
-          pr_tma<CG>(sk + st * Cfg::kK + piece * (Cfg::kBoxK * 128) + c * p.box_k * 128, &kmap, row,
-                     kv_head * Cfg::kPieces + piece, smem_u32(&k_full[st]) & (CG == 2 ? kLeaderMask : 0xffffffffu));
-        }
-        // V: every key, this CTA's pieces
-        if (ph > 0) ok = pr_wait(&v_empty[st], uint32_t(ph - 1) & 1u, p.a.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int cv = (n + p.box_v - 1) / p.box_v;
-        if (lane == 0) mbar_expect_tx(&v_full[st], uint32_t(cv * p.box_v * Cfg::kPiecesV * 128));
-        __syncwarp();
-        for (int i = lane; i < cv * Cfg::kPiecesV; i += 32) {
-          const int c = i / Cfg::kPiecesV, piece = i % Cfg::kPiecesV;
-          const int row = row_of(k0 + c * p.box_v);
-          pr_tma<CG>(sv + st * Cfg::kK + piece * (PR_KEYS * 128) + c * p.box_v * 128, &vmap, row,
-                     kv_head * Cfg::kPieces + int(rank) * Cfg::kPiecesV + piece, smem_u32(&v_full[st]));
+        if (i > 0) {  // V: every key, this CTA's pieces
+          const int k0 = g.key0 + (i - 1) * PR_KEYS, n = min(PR_KEYS, g.key_hi - k0);
+          ok = pr_wait(&v_empty[v_st], v_ph, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int cv = (n + bv - 1) >> p.box_v;
+          if (elect_one()) mbar_expect_tx(&v_full[v_st], uint32_t(cv * bv * Cfg::kPiecesV * 128));
+          __syncwarp();
+          const int row = lane < cv ? row_of(k0 + lane * bv) : 0;
+          for (int c = 0; c < cv; ++c) {
+            const int r = __shfl_sync(0xffffffffu, row, c);
+            if (elect_one()) {
+#pragma unroll
+              for (int piece = 0; piece < Cfg::kPiecesV; ++piece)
+                pr_tma<CG>(sv + v_st * Cfg::kK + piece * (PR_KEYS * 128) + c * bv * 128, &vmap, r,
+                           it.head * Cfg::kPieces + int(rank) * Cfg::kPiecesV + piece, smem_u32(&v_full[v_st]));
+            }
+            __syncwarp();
+          }
+          if (++v_st == ST) v_st = 0, v_ph ^= 1u;
         }
       }
-      // the copies that nobody else waits for: after a timeout, all in flight
-      if (!ok)
-        for (int i = 0; i < ST; ++i) {
-          if (rank == 0) mbar_wait_parity_sleep(&k_full[i], 0, p.a.err);
-          mbar_wait_parity_sleep(&v_full[i], 0, p.a.err);
-        }
-    } else if (warp == ISSUER) {
-      // ---- one thread of the pair's first CTA issues every product
-      if (rank == 0 && lane == 0 && ntiles > 0) {
-        constexpr uint32_t id_qk = pr_idesc(FMT, PR_ROWS * CG, PR_KEYS, 0), id_pv = pr_idesc(FMT, PR_ROWS * CG, D, 1);
-        const int units = ntiles * NQ;
-        const auto qk = [&](int u) {
-          const int j = u / NQ, q = u % NQ, st = j % ST;
-          if (q == 0) ok = ok && pr_wait(&k_full[st], uint32_t(j / ST) & 1u, p.a.err);
-          if (!ok) return;
-          tc_after();
+      if (!ok) break;
+    }
+    // after a timeout: the copies that nobody else waits for
+    if (!ok)
+      for (int i = 0; i < ST; ++i) {
+        if (rank == 0) pr_wait(&k_full[i], k_ph, nullptr);
+        pr_wait(&v_full[i], v_ph, nullptr);
+      }
+  } else if (warp == ISSUER || (Cfg::kOwnP && warp == ISSUER_O)) {
+    // ---- the products, issued by one thread of the pair's first CTA.  What
+    // an issuer does between a barrier and its product is on every tile's path
+    // (all its waits and descriptors took over 1000 clocks a tile, as
+    // long as the products of head_dim 128), so everything else is waited for first.
+    constexpr uint32_t id_qk = pr_idesc(FMT, PR_ROWS * CG, PR_KEYS, 0), id_pv = pr_idesc(FMT, PR_ROWS * CG, D, 1);
+    int k_st = 0, v_st = 0;
+    uint32_t k_ph = 0, v_ph = 0, sn = 0, on = 0;  // stages of K and V, their parities; S and O products so far
+    uint32_t nq = 0;                              // items with rows so far
+    const auto issue_s = [&](bool last) {
+      tc_after();
+      if (elect_one()) {
+        const uint64_t a = pr_desc(sq, 16, 1024), b = pr_desc(sk + k_st * Cfg::kK, 16, 1024);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            pr_mma_ss<CG>(tmem + uint32_t(u & 1) * 128,
-                          pr_desc(sq + q * Cfg::kQ + (k >> 2) * (PR_ROWS * 128) + (k & 3) * 32, 16, 1024),
-                          pr_desc(sk + st * Cfg::kK + (k >> 2) * (Cfg::kBoxK * 128) + (k & 3) * 32, 16, 1024), id_qk, k > 0);
-          pr_commit<CG>(&s_full[u & 1]);
-          if (q == NQ - 1) pr_commit<CG>(&k_empty[st]);
-        };
-        ok = pr_wait(&q_full, 0, p.a.err);
-        qk(0);
-        for (int u = 0; u < units && ok; ++u) {
-          if (u + 1 < units) qk(u + 1);
-          const int j = u / NQ, q = u % NQ, st = j % ST;
-          ok = ok && pr_wait(&p_ready[u & 1], uint32_t(u >> 1) & 1u, p.a.err);
-          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
-          if (!ok) break;
-          tc_after();
-#pragma unroll
-          for (int k = 0; k < PR_KEYS / 16; ++k)
-            pr_mma_ts<CG>(tmem + Cfg::kTmemO + q * D, tmem + uint32_t(u & 1) * 128 + k * 8,
-                          pr_desc(sv + st * Cfg::kK + k * 2048, PR_KEYS * 128, 1024), id_pv, j > 0 || k > 0);
-          pr_commit<CG>(&pv_done[u & 1]);
-          if (q == NQ - 1) pr_commit<CG>(&v_empty[st]);
-        }
+        for (int k = 0; k < D / 16; ++k)
+          pr_mma_ss<CG>(tmem + (sn & 1) * 128, a + ((k >> 2) * (PR_ROWS * 128) + (k & 3) * 32) / 16,
+                        b + ((k >> 2) * (Cfg::kKeys * 128) + (k & 3) * 32) / 16, id_qk, k > 0);
+        pr_commit<CG>(&s_full[sn & 1]);
+        pr_commit<CG>(&k_empty[k_st]);
+        if (last) pr_commit<CG>(&q_free);
       }
       __syncwarp();
-    } else {
-      // ---- softmax: thread = row of row tile q, half `half` of its columns
-      const int q = warp >> 3, half = (warp >> 2) & 1, lt = t & 127, lt2 = t & 255;
-      const uint32_t lanes = uint32_t(warp & 3) * 32u << 16;
-      const int pair_bar = 1 + q * 4 + (warp & 3);  // the two warps that share 32 rows
-      const int rt = r0 + (int(rank) * NQ + q) * PR_ROWS;  // the tile's first row
-      const int r = rt + lt;
-      const bool live = r < nrows;
-      const int pos = pos0 + (live ? r : nrows - 1) / group;
-      const int lim = live ? min(pos, sp.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
-      // keys [all_lo, all_hi] are seen by every row of the tile
-      const int all_hi = min(sp.len - 1, pos0 + min(rt, nrows - 1) / group);
-      const int all_lo = window > 0 ? pos0 + min(rt + PR_ROWS - 1, nrows - 1) / group - window + 1 : 0;
-      const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
-      // Rows of the tile to (token, head of the group): row rr is pair
-      // rem + rr counted from token tok0, divided by a multiplication (exact
-      // below 2^21 / group, and rem + rr < 1152)
-      const int tok0 = rt / group, rem = rt - tok0 * group;
-      const uint32_t inv_group = ((1u << 21) + uint32_t(group) - 1u) / uint32_t(group);
-      const auto row_at = [&](int rr) {  // element offset of the row's head in a [row][heads][D] tensor, less the token's
-        const int x = rem + rr, tok = int((uint32_t(x) * inv_group) >> 21);
-        return make_int2(sp.row0 + tok0 + tok, kv_head * group + x - tok * group);
-      };
-      // Q into the swizzled operand layout, 16 bytes at a time, neighbouring
-      // lanes neighbouring bytes of a row, eight loads in flight per thread.
-      // A negative scale flips Q's sign.
-      {
-        const uint32_t flip = p.a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-        constexpr int N = PR_ROWS * (D / 8) / 256, B = N < 8 ? N : 8;
-#pragma unroll 1
-        for (int i0 = 0; i0 < N; i0 += B) {
-          uint4 v[B];
+      ++sn;
+      if (++k_st == ST) k_st = 0, k_ph ^= 1u;
+    };
+    const auto issue_o = [&](const PrGeom& g, int o) {
+      // keys behind the last one in use are not multiplied, 16 at a time
+      const int steps = (min(PR_KEYS, g.key_hi - g.key0 - o * PR_KEYS) + 15) / 16;
+      tc_after();
+      if (elect_one()) {
+        const uint32_t a = tmem + Cfg::p_col(on & 1);
+        const uint64_t b = pr_desc(sv + v_st * Cfg::kK, PR_KEYS * 128, 1024);
+        pr_mma_ts<CG>(tmem + Cfg::kTmemO, a, b, id_pv, o > 0);
+        if (steps == PR_KEYS / 16) {
 #pragma unroll
-          for (int i = 0; i < B; ++i) {
-            const int at = (i0 + i) * 256 + lt2, rr = at / (D / 8), c = at % (D / 8);
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (rt + rr < nrows && ntiles > 0) {
-              const int2 w = row_at(rr);
-              v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + int64_t(w.x) * p.a.q_stride + w.y * D +
-                                                     c * 8);
-            }
+          for (int k = 1; k < PR_KEYS / 16; ++k) pr_mma_ts<CG>(tmem + Cfg::kTmemO, a + k * 8, b + k * (2048 / 16), id_pv, true);
+        } else {
+          for (int k = 1; k < steps; ++k) pr_mma_ts<CG>(tmem + Cfg::kTmemO, a + k * 8, b + k * (2048 / 16), id_pv, true);
+        }
+        pr_commit<CG>(&pv_done[on & 1]);
+        pr_commit<CG>(&v_empty[v_st]);
+      }
+      __syncwarp();
+      ++on;
+      if (++v_st == ST) v_st = 0, v_ph ^= 1u;
+    };
+    const auto wait_v = [&] {
+      return CG == 2 ? pr_wait2(&v_full[v_st], v_ph, &v_peer[v_st], v_ph, err) : pr_wait(&v_full[v_st], v_ph, err);
+    };
+    PrItem it;
+    for (int n_it = 0; next_item(n_it, &it); ++n_it) {
+      const PrGeom g = pr_geom(it, group, window, SPAN);
+      if (g.units == 0) continue;
+      if (rank != 0) {  // the second CTA reports its half of every V tile
+        if (warp == ISSUER)
+          for (int i = 0; i < g.units; ++i) {
+            ok = ok && pr_wait(&v_full[v_st], v_ph, err);
+            __syncwarp();
+            if (lane == 0 && ok) arrive_leader<CG>(&v_peer[v_st]);
+            if (++v_st == ST) v_st = 0, v_ph ^= 1u;
           }
-#pragma unroll
-          for (int i = 0; i < B; ++i) {
-            const int at = (i0 + i) * 256 + lt2, rr = at / (D / 8), c = at % (D / 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + q * Cfg::kQ + (c >> 3) * (PR_ROWS * 128) +
-                                                                         rr * 128 + (((c & 7) ^ (rr & 7)) << 4)),
-                         "r"(v[i].x ^ flip), "r"(v[i].y ^ flip), "r"(v[i].z ^ flip), "r"(v[i].w ^ flip)
-                         : "memory");
+        continue;
+      }
+      if (warp == ISSUER) {
+        ok = ok && pr_wait(&q_full, nq & 1u, err);
+        if (nq == 0) ok = ok && pr_wait(&q_first, 0, err);
+      }
+      if constexpr (Cfg::kOwnP) {
+        // S and O each by a warp of their own: all that orders them are the slots
+        if (warp == ISSUER) {
+          for (int i = 0; i < g.units; ++i) {
+            if (sn >= 2) ok = ok && pr_wait2(&k_full[k_st], k_ph, &s_free[sn & 1], ((sn >> 1) - 1) & 1u, err);
+            else ok = ok && pr_wait(&k_full[k_st], k_ph, err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            issue_s(i + 1 == g.units);
+          }
+        } else {
+          if (nq > 0) ok = ok && pr_wait(&o_free, (nq - 1) & 1u, err);
+          for (int o = 0; o < g.units; ++o) {
+            ok = ok && wait_v() && pr_wait(&p_ready[on & 1], (on >> 1) & 1u, err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            issue_o(g, o);
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(&q_full);
+      } else {
+        // P lies in its S slot, so S of tile o + 2 has to be issued behind O of
+        // tile o, by the same thread
+        ok = ok && pr_wait(&k_full[k_st], k_ph, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) issue_s(g.units == 1);
+        if (ok && g.units > 1) {
+          ok = pr_wait(&k_full[k_st], k_ph, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) issue_s(g.units == 2);
+        }
+        if (nq > 0) ok = ok && pr_wait(&o_free, (nq - 1) & 1u, err);
+        for (int o = 0; o < g.units && ok; ++o) {
+          ok = wait_v();
+          if (o + 2 < g.units) ok = ok && pr_wait2(&k_full[k_st], k_ph, &p_ready[on & 1], (on >> 1) & 1u, err);
+          else ok = ok && pr_wait(&p_ready[on & 1], (on >> 1) & 1u, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          issue_o(g, o);
+          if (o + 2 < g.units) issue_s(o + 3 == g.units);
+        }
       }
-      constexpr int HC = PR_KEYS / 2;  // columns of a half
+      if (!ok) break;
+      ++nq;
+    }
+  } else {
+    // ---- items: the sequences' tiles in order, each sequence's last rows
+    // (the longest sums) first, the KV heads of a tile side by side; and
+    // the Q of every item but the first
+    const auto tiles = [&](const SeqSpan& q) { return (q.n * group + SPAN - 1) / SPAN * p.a.kv_heads; };
+    int s0 = 0, before = 0;  // items of the sequences before s0
+    int x = int(blockIdx.x) / CG;
+    int nq = 0;
+    const int l64 = t - 32 * SCHEDULER;
+    for (int n_it = 0; ok; ++n_it) {
+      PrItem it;
+      it.seq = -1;
+      if (warp == SCHEDULER) {
+        if (n_it > 0) {
+          // the answer to the request made when the last item went out
+          ok = pr_wait(&clc_full, uint32_t(n_it - 1) & 1u, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int first = clc_answer(&clc_resp);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          x = first < 0 ? -1 : first / CG;
+          __syncwarp();
+        }
+        if (x < before) s0 = before = 0;  // items come in launch order, but nothing promises it
+        while (x >= 0 && s0 < p.b.seqs) {  // 32 sequences at a time
+          SeqSpan own{};
+          bool bad = false;
+          if (s0 + lane < p.b.seqs) own = seq_span(p.b, s0 + lane, &bad);
+          if (bad && err) atomicExch(err, DEVICE_ERR_PAGE);
+          const int mine = tiles(own);
+          int incl = mine;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += v;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, x < before + incl);
+          if (hit) {
+            const int w = __ffs(hit) - 1;
+            const int at = x - before - __shfl_sync(0xffffffffu, incl - mine, w), n = __shfl_sync(0xffffffffu, mine, w);
+            it.span.row0 = __shfl_sync(0xffffffffu, own.row0, w);
+            it.span.n = __shfl_sync(0xffffffffu, own.n, w);
+            it.span.len = __shfl_sync(0xffffffffu, own.len, w);
+            it.seq = s0 + w;
+            it.head = at % p.a.kv_heads;
+            it.tile = n / p.a.kv_heads - 1 - at / p.a.kv_heads;
+            break;
+          }
+          before += __shfl_sync(0xffffffffu, incl, 31);
+          s0 += 32;
+        }
+        if (n_it >= 2) {
+          ok = pr_wait(&item_empty[n_it & 1], uint32_t((n_it >> 1) - 1) & 1u, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        if (lane == 0) {
+          s_items[n_it & 1] = it;
+          mbar_arrive(&item_full[n_it & 1]);
+          if (it.seq >= 0) {
+            // a pair's first CTA asks for both, once the other has read the last answer
+            mbar_expect_tx(&clc_full, 16);
+            if (CG == 2 && rank == 1) arrive_leader<CG>(&clc_ready);
+            if (rank == 0) {
+              if (CG == 2) ok = pr_wait(&clc_ready, uint32_t(n_it) & 1u, err);
+              if (ok) clc_ask<CG>(&clc_resp, &clc_full);
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || it.seq < 0) break;
+      } else if (!next_item(n_it, &it)) {
+        break;
+      }
+      const PrGeom g = pr_geom(it, group, window, SPAN);
+      if (g.units > 0) {
+        if (n_it > 0) {
+          if (nq > 0) ok = pr_wait(&q_free, uint32_t(nq - 1) & 1u, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          load_q(it, g, l64, 32 * LOADERS);
+        }
+        if (lane == 0) arrive_leader<CG>(&q_full);
+        ++nq;
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
+    // ---- softmax: thread = row; warpgroup wg takes the tiles whose number is
+    // of its parity (over all items)
+    const int wg = warp >> 2, w4 = warp & 3, lt = t & 127;
+    const uint32_t lanes = uint32_t(w4) * 32u << 16;
+    const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
+    uint32_t v0 = 0;    // tiles before this item
+    uint32_t ends = 0;  // items with tiles so far
+    const uint32_t sa = tmem + lanes + uint32_t(wg) * 128, pa = tmem + lanes + Cfg::p_col(uint32_t(wg));
+    const uint32_t oa = tmem + lanes + Cfg::kTmemO;
+    PrItem it;
+    for (int n_it = 0; next_item(n_it, &it); ++n_it) {
+      const PrGeom g = pr_geom(it, group, window, SPAN);
+      const int rt = g.r0 + int(rank) * PR_ROWS;  // the CTA's first row
+      const int tok0 = rt / group, rem = rt - tok0 * group;
+      const bool live = rt + lt < g.nrows;
+      if (n_it == 0) {
+        if (g.units > 0) load_q(it, g, t, 256);
+        if (lane == 0) arrive_leader<CG>(&q_first);
+      }
+      const int2 own = row_at(tok0, rem, live ? lt : 0);  // token, head of the group
+      const int pos = g.pos0 + own.x;
+      const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
+      // keys [all_lo, all_hi] are seen by every row of the item (in a pair
+      // each CTA looks after half of every value for both)
+      const int all_hi = min(it.span.len - 1, g.pos0 + g.r0 / group);
+      const int all_lo = window > 0 ? g.pos0 + (min(g.r0 + SPAN, g.nrows) - 1) / group - window + 1 : 0;
       float m = -INFINITY, l = 0.0f;
-      for (int j = 0; j < ntiles; ++j) {
-        const int u = j * NQ + q, buf = u & 1, st = j % ST, k0 = (tile0 + j) * PR_KEYS;
-        ok = ok && pr_wait(&s_full[buf], uint32_t(u >> 1) & 1u, p.a.err);
+      for (int u = int((v0 ^ uint32_t(wg)) & 1u); u < g.units; u += 2) {
+        const uint32_t v = v0 + uint32_t(u);
+        const int k0 = g.key0 + u * PR_KEYS;
+        ok = ok && pr_wait(&s_full[wg], (v >> 1) & 1u, err);
         __syncwarp();
         tc_after();
-        uint32_t s[HC];
-        const uint32_t sa = tmem + lanes + uint32_t(buf) * 128;
+        uint32_t s[PR_KEYS];
 #pragma unroll
-        for (int c = 0; c < HC; c += 32) tm_ld32(sa + half * HC + c, s + c);
+        for (int c = 0; c < PR_KEYS; c += 32) tm_ld32(sa + c, s + c);
         tm_wait_ld();
+        if constexpr (Cfg::kOwnP) {
+          tc_before();
+          __syncwarp();
+          if (lane == 0 && ok) arrive_leader<CG>(&s_free[wg]);
+        }
         const bool edge = k0 + PR_KEYS - 1 > all_hi || k0 < all_lo;
         if (edge) {
-          const int hi = lim - k0 - half * HC, lo = low - k0 - half * HC;
+          const int hi = lim - k0, lo = low - k0;
 #pragma unroll
-          for (int c = 0; c < HC; ++c)
+          for (int c = 0; c < PR_KEYS; ++c)
             if (c > hi || c < lo) s[c] = 0xff800000u;
         }
         float mx[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
+        for (int e = 0; e < 4; ++e) mx[e] = max3(__uint_as_float(s[e]), __uint_as_float(s[4 + e]), __uint_as_float(s[8 + e]));
 #pragma unroll
-        for (int c = 4; c + 4 < HC; c += 8)
+        for (int c = 12; c + 8 <= PR_KEYS; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + e]), __uint_as_float(s[c + 4 + e])));
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(s[c + e]), __uint_as_float(s[c + 4 + e]));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[HC - 4 + e]));
-        float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // the other half's maximum: one exchange between the two warps of the
-        // rows (the slot alternates, so the next one need not wait for readers)
-        s_half[j & 1][half][q * PR_ROWS + lt] = mt;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-        mt = fmaxf(mt, s_half[j & 1][half ^ 1][q * PR_ROWS + lt]);
-        const bool grew = mt > m && !((mt - m) * sc <= PR_GROW);  // m = -inf included
-        if (__any_sync(0xffffffffu, grew)) {
-          const float f = grew ? ex2((m - mt) * sc) : 1.0f;
-          if (grew) m = mt;
-          l *= f;
-          if (j > 0) {
-            const int up = u - NQ;  // the tile's previous product must have landed
-            ok = ok && pr_wait(&pv_done[up & 1], uint32_t(up >> 1) & 1u, p.a.err);
-            __syncwarp();
-            tc_after();
-            const uint32_t oa = tmem + lanes + Cfg::kTmemO + uint32_t(q * D + half * (D / 2));
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(s[PR_KEYS - 4 + e]), mx[e]);
+        float mt = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
+        // a score of +inf makes the row NaN (inf - inf), as a NaN does
+        if (mt == INFINITY) mt = __int_as_float(0x7fffffff);
+        // m as the other warpgroup left it at the tile before, and on to the next
+        float now = -INFINITY;
+        if (u > 0) {
+          ok = ok && pr_wait(&m_pass[w4], (v - 1) & 1u, err);
+          __syncwarp();
+          now = s_m[lt];
+        }
+        const bool grew = !(mt <= now) && !((mt - now) * sc <= PR_GROW);  // now = -inf and NaN included
+        const float f = grew ? ex2((now - mt) * sc) : 1.0f;
+        if (grew) now = mt;
+        s_m[lt] = now;
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(&m_pass[w4]);
+        if (now != m) {  // (l is 0 as long as m is -inf)
+          l *= ex2((m - now) * sc);
+          m = now;
+        }
+        if (__any_sync(0xffffffffu, grew) && u > 0) {
+          // O to the new m, once the product before has landed
+          ok = ok && pr_wait(&pv_done[wg ^ 1], ((v - 1) >> 1) & 1u, err);
+          __syncwarp();
+          tc_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
-              uint32_t o[16];
-              tm_ld16(oa + c, o);
-              tm_wait_ld();
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tm_ld16(oa + c, o);
+            tm_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tm_st16(oa + c, o);
-            }
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tm_st16(oa + c, o);
           }
+        }
+        if constexpr (Cfg::kOwnP) {  // the P slot: the product that read it last
+          if (v >= 2) ok = ok && pr_wait(&pv_done[wg], ((v >> 1) - 1) & 1u, err);
+          __syncwarp();
+          tc_after();
         }
         const float ms = m == -INFINITY ? 0.0f : m * sc;
         const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(-ms, -ms);
         uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-        uint32_t pk[HC / 2];
+        const auto exps = [&](auto poly) {
 #pragma unroll
-        for (int c = 0; c < HC; c += 2) {
-          const uint64_t x = fma2(pack2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nm2);
-          float a, b;
-          unpack2(x, a, b);
-          a = ex2(a), b = ex2(b);
-          sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(a, b));
-          pk[c >> 1] = HalfOps<T>::pack(a, b);
-        }
-        // P takes the first half of S's columns: the other warp's scores are
-        // read (the exchange above came after both loads)
-        tm_st32(sa + half * (HC / 2), pk);
+          for (int b = 0; b < PR_KEYS; b += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const uint64_t x = fma2(pack2(__uint_as_float(s[b + c]), __uint_as_float(s[b + c + 1])), sc2, nm2);
+              float e0, e1;
+              if (poly.value && (c >> 1) % PR_POLY_EVERY == PR_POLY_EVERY - 1) {
+                ex2_poly2(x, e0, e1);
+              } else {
+                unpack2(x, e0, e1);
+                e0 = ex2(e0), e1 = ex2(e1);
+              }
+              sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(e0, e1));
+              pk[c >> 1] = HalfOps<T>::pack(e0, e1);
+            }
+            tm_st16(pa + b / 2, pk);
+          }
+        };
+        if (edge) exps(std::false_type{});  // -inf has to give 0
+        else exps(std::true_type{});
         {
           float a, b;
           unpack2(add2(sum[0], sum[1]), a, b);
           l += a + b;
         }
         if (edge) {
-          // values of keys behind the end, and values that only some rows see
-          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
+          // values of keys that no row uses, and values that only some rows see
+          const uint32_t st = v % ST, vt = sv + st * Cfg::kK;
+          ok = ok && pr_wait(&v_full[st], (v / ST) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
-          const uint32_t vt = sv + st * Cfg::kK;
           bool odd = false;
           if (ok)
-            for (int i = lt2; i < PR_KEYS * Cfg::kPiecesV * 8; i += 256) {
+            for (int i = lt; i < PR_KEYS * Cfg::kPiecesV * 8; i += 128) {
               const int key = i / (Cfg::kPiecesV * 8), c = i % (Cfg::kPiecesV * 8);
               const uint32_t at = vt + (c >> 3) * (PR_KEYS * 128) + key * 128 + ((c & 7) << 4);
-              if (k0 + key >= sp.len) {
+              if (k0 + key >= g.key_hi) {
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
               } else {
                 uint32_t a, b, d, e;
@@ -658,119 +975,136 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           if (__any_sync(0xffffffffu, odd) && lane == 0) {
             // both CTAs' rows are the sums of both CTAs' dims
-            if constexpr (CG == 1) {
-              atomicExch(&s_odd, 1);
-            } else {
-              for (int c = 0; c < CG; ++c)
+            for (int c = 0; c < CG; ++c) {
+              if constexpr (CG == 1)
+                atomicExch(&s_odd[n_it & 3], n_it + 1);
+              else
                 asm volatile(
                     "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\tst.shared::cluster.u32 [ra], %2;\n\t}\n" ::"r"(
-                        smem_u32(&s_odd)),
-                    "r"(c), "r"(1)
+                        smem_u32(&s_odd[n_it & 3])),
+                    "r"(c), "r"(n_it + 1)
                     : "memory");
             }
           }
           // what was written here is read by the pair's products
           if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-        } else if (CG == 2) {
-          // the issuer sees only its own CTA's V barrier: a CTA's arrival on
-          // p_ready also says that its half of V has landed
-          ok = ok && pr_wait(&v_full[st], uint32_t(j / ST) & 1u, p.a.err);
-          __syncwarp();
         }
         tm_wait_st();
         tc_before();
-        // a warp whose wait gave up walks on without arriving, to meet the
-        // other warp at the exchanges; nothing after it completes
-        ok = __all_sync(0xffffffffu, ok);
-        if (lane == 0 && ok) arrive_leader<CG>(&p_ready[buf]);
+        __syncwarp();
+        if (lane == 0 && ok) arrive_leader<CG>(&p_ready[wg]);
       }
-      // ---- the rows' outputs
-      if (ntiles > 0) {
-        const int ul = (ntiles - 1) * NQ + q;
-        ok = ok && pr_wait(&pv_done[ul & 1], uint32_t(ul >> 1) & 1u, p.a.err);
-        ok = __all_sync(0xffffffffu, ok);
+      v0 += uint32_t(g.units);
+      // ---- the rows' outputs: both warpgroups' sums, and O once the last
+      // product has landed (the one two before it has: its slot was used again)
+      if (g.units > 0) {
+        s_l[ends & 1][wg][lt] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_pass[w4]);
+        ok = ok && pr_wait(&l_pass[w4], ends & 1u, err);
+        __syncwarp();
+        const float2 a = s_l[ends & 1][0][lt], b = s_l[ends & 1][1][lt];
+        m = fmaxf(a.x, b.x);
+        l = m == -INFINITY ? a.y + b.y : a.y * ex2((a.x - m) * sc) + b.y * ex2((b.x - m) * sc);
+        ok = ok && pr_wait(&pv_done[(v0 - 1) & 1], ((v0 - 1) >> 1) & 1u, err);
+        __syncwarp();
         tc_after();
+        ++ends;
       }
-      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");  // the last maxima are read
-      s_half[0][half][q * PR_ROWS + lt] = l;
-      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-      l = s_half[0][0][q * PR_ROWS + lt] + s_half[0][1][q * PR_ROWS + lt];
-      if (ok) {
-        const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-        const int2 own = row_at(live ? lt : 0);
-        const int64_t row = int64_t(own.x) * p.a.heads + own.y;
-        float* lse = p.a.lse ? p.a.lse + row : nullptr;
-        if (ntiles > 0 && *static_cast<volatile int*>(&s_odd)) {
-          if (live && half == 0)
-            pr_plain_row<T, D>(p, seq, sp.row0, kv_head, static_cast<const T*>(p.a.q) + int64_t(own.x) * p.a.q_stride + own.y * D,
-                               max(low, 0), lim, static_cast<T*>(p.a.out) + row * D,
-                               p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr, lse);
-        } else {
-          // through shared memory (the operands are done with), so that a warp
-          // stores whole rows: 16-byte chunk c of row rr at chunk c ^ (rr % 8)
-          const int chunks = p.a.out_f32 ? D / 4 : D / 8;  // 16-byte chunks of a row
-          const uint32_t stage = base + uint32_t(q * PR_ROWS) * chunks * 16;
-#pragma unroll 1
-          for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-            uint32_t o[32];
-            if (ntiles > 0) {
-              tm_ld32(tmem + lanes + Cfg::kTmemO + uint32_t(q) * D + c, o);
-              tm_wait_ld();
-            } else {
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+      const int64_t row = int64_t(it.span.row0 + own.x) * p.a.heads + it.head * group + own.y;
+      float* lse = p.a.lse ? p.a.lse + row : nullptr;
+      const bool odd = g.units > 0 && *static_cast<volatile int*>(&s_odd[n_it & 3]) == n_it + 1;
+      if (live && lse && wg == 0 && !odd) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
+      // 64 bytes of each of the warp's 32 rows at a time through shared
+      // memory, so that four lanes store 64 consecutive bytes: 16-byte chunk c of
+      // row r at chunk c ^ (r / 2 % 4)
+      const uint32_t stage = so + uint32_t(warp) * 2048;
+      const auto put = [&](int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)), "r"(a),
+                     "r"(b), "r"(d), "r"(e)
+                     : "memory");
+      };
+      const int esz = p.a.out_f32 ? 4 : 2;
+      uint8_t* dst[4];  // this lane's 16 bytes of four rows, column 0; nullptr: no row
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = 0;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
-            const auto put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (lt * chunks + (chunk ^ (lt & 7))) * 16), "r"(x),
-                           "r"(y), "r"(z), "r"(w)
-                           : "memory");
-            };
-            if (p.a.out_f32) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) put((c + e) / 4, o[e], o[e + 1], o[e + 2], o[e + 3]);
-            } else {
-              uint32_t w[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                w[e] = HalfOps<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-#pragma unroll
-              for (int e = 0; e < 16; e += 4) put((c + 2 * e) / 8, w[e], w[e + 1], w[e + 2], w[e + 3]);
-            }
-          }
-          if (live && lse && half == 0) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int rr = w4 * 32 + i * 8 + (lane >> 2);
+        const int2 w = row_at(tok0, rem, rr);
+        const int64_t at = (int64_t(it.span.row0 + w.x) * p.a.heads + it.head * group + w.y) * D;
+        dst[i] = rt + rr < g.nrows && !odd ? static_cast<uint8_t*>(p.a.out) + at * esz + (lane & 3) * 16 : nullptr;
       }
-      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-      if (ok && !(ntiles > 0 && *static_cast<volatile int*>(&s_odd))) {
-        // the two warps of these 32 rows store 16 rows each
-        const int chunks = p.a.out_f32 ? D / 4 : D / 8;
-        const uint32_t stage = base + uint32_t(q * PR_ROWS) * chunks * 16;
-        const int first = (warp & 3) * 32 + half * 16;
-        const int shift = 31 - __clz(chunks);
-#pragma unroll 4
-        for (int i = lane; i < 16 * chunks; i += 32) {
-          const int rr = first + (i >> shift), c = i & (chunks - 1);
-          if (rt + rr >= nrows) break;
-          uint4 v;
+      const auto flush = [&](int col) {  // the staged bytes start at column col
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = i * 8 + (lane >> 2), c = lane & 3;
+          uint4 x;
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                       : "r"(stage + (rr * chunks + (c ^ (rr & 7))) * 16)
+                       : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                       : "r"(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4))
                        : "memory");
-          const int2 w = row_at(rr);
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.a.out) + ((int64_t(w.x) * p.a.heads + w.y) * chunks + c) * 16) = v;
+          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + col * esz) = x;
+        }
+        __syncwarp();
+      };
+#pragma unroll 1
+      for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
+        uint32_t o[32];
+        if (g.units > 0) {
+          tm_ld32(oa + c, o);
+          tm_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+        if (p.a.out_f32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              put(e, o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
+            flush(c + 16 * h);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = HalfOps<T>::pack(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
+            put(e, w[0], w[1], w[2], w[3]);
+          }
+          flush(c);
         }
       }
-      // after a timeout the products in flight get one more bounded wait
-      // before the tensor memory is freed
-      if (!ok) {
-        pr_wait(&s_full[0], 0, nullptr);
-        pr_wait(&pv_done[0], 0, nullptr);
+      if (g.units > 0) {  // the next item's first product may overwrite O
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader<CG>(&o_free);
       }
-      __syncwarp();
+      if (odd) {
+        if (live && wg == 0)
+          pr_plain_row<T, D>(p, it.seq, it.span.row0, it.head,
+                             static_cast<const T*>(p.a.q) + int64_t(it.span.row0 + own.x) * p.a.q_stride +
+                                 (it.head * group + own.y) * D,
+                             max(low, 0), lim, static_cast<T*>(p.a.out) + row * D,
+                             p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr, lse);
+        __syncwarp();
+      }
+    }
+    // after a timeout the products in flight get one more bounded wait before
+    // the tensor memory is freed
+    if (!ok) {
+      pr_wait(&s_full[0], 0, nullptr);
+      pr_wait(&pv_done[0], 0, nullptr);
     }
   }
+  __syncwarp();
   tc_before();
   sync_all<CG>();
   tc_after();
@@ -790,16 +1124,17 @@ cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, cudaStream_t st) {
   });
   if (e != cudaSuccess) return e;
   const int page = 1 << p.b.page_shift;
-  p.box_k = p.b.table ? std::min(Cfg::kBoxK, page) : Cfg::kBoxK;
-  p.box_v = p.b.table ? std::min(PR_KEYS, page) : PR_KEYS;
+  const int bk = p.b.table ? std::min(Cfg::kKeys, page) : Cfg::kKeys, bv = p.b.table ? std::min(PR_KEYS, page) : PR_KEYS;
+  p.box_k = __builtin_ctz(bk);
+  p.box_v = __builtin_ctz(bv);
   p.slots = int64_t(kv.slots);
   CUtensorMap km, vm;
-  e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, p.box_k, 1);
+  e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, bk, 1);
   if (e == cudaSuccess)
-    e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, p.box_v, 1);
+    e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, bv, 1);
   if (e != cudaSuccess) return e;
   // every sequence adds at most one tile to those of the rows put together
-  constexpr int SPAN = PR_ROWS * Cfg::NQ * Cfg::CG;
+  constexpr int SPAN = PR_ROWS * Cfg::CG;
   const int group = p.a.heads / p.a.kv_heads;
   const int64_t items =
       (int64_t(p.b.rows) * group / SPAN + std::min(p.b.seqs, p.b.rows)) * p.a.kv_heads;

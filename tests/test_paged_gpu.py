@@ -137,6 +137,25 @@ def test_packed_prompts(dim, dtype, heads, kv_heads, new, window):
     _check(got, lse, b, b.q, dim ** -0.5, window)
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads,window", [(64, 16, 8, 0), (128, 8, 8, 50), (256, 12, 6, 0)])
+def test_more_tiles_than_the_machine_holds_at_once(dim, heads, kv_heads, window):
+    # several times the tiles of one wave, of all lengths, among them sequences
+    # without keys, and rows before the first key
+    g = torch.Generator().manual_seed(dim)
+    new = torch.randint(0, 500, (60,), generator=g).tolist()
+    past = [(-20, 0, 0, 130, 411)[i % 5] if n else 0 for i, n in enumerate(new)]
+    lens = [max(0, n + p) for n, p in zip(new, past)]
+    b = ref.Batch(new, lens, kv_heads, dim, 16, torch.bfloat16)
+    q = _q(b, heads, dim, torch.bfloat16)
+    for rep in range(3):
+        got, lse = hk.paged_attention(q, b.key, b.value, b.table, b.query_starts, b.kv_lens, max_query_len=500,
+                                      scale=-(dim ** -0.5), window=window, return_lse=True)
+        if rep == 0:
+            _check(got, lse, b, q, -(dim ** -0.5), window)
+            first = got
+        assert torch.equal(got, first)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("new,past", [(1, 77), (5, 60), (150, 0), (150, 70)])
 def test_values_that_are_not_finite_reach_only_rows_that_see_them(dim, new, past):
