@@ -83,6 +83,7 @@ struct PrArgs {
   const void* v;
   int64_t k_stride, v_stride;
   int box_k, box_v;    // key rows per TMA copy, as powers of two
+  int whole_k, whole_v;  // a copy brings the CTA's whole tile, every piece of it
   int64_t slots;
 };
 
@@ -259,11 +260,12 @@ __device__ __forceinline__ bool pr_try(uint64_t* bar, uint32_t parity) {
                : "memory");
   return ok != 0;
 }
-// mbar_wait_parity without a timer read where the phase is already complete.
-__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err) {
+// The rest of a wait, bounded in time.
+__device__ __forceinline__ bool pr_wait_on(uint64_t* bar, uint32_t parity, int* err) {
   unsigned long long t0 = 0;
   for (int it = 0;; ++it) {
     if (pr_try(bar, parity)) return true;
+    if (it & 15) continue;
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     if (it == 0) {
@@ -274,11 +276,16 @@ __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err
     }
   }
 }
+// A bounded wait (as mbar_wait_parity) that costs one instruction's round trip
+// where the phase is already complete.
+__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return pr_try(bar, parity) || pr_wait_on(bar, parity, err);
+}
 // Two barriers with their answers in flight together: the common case, both
 // complete, costs one round trip instead of two.
 __device__ __forceinline__ bool pr_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* err) {
   const bool x = pr_try(a, pa), y = pr_try(b, pb);
-  return (x || pr_wait(a, pa, err)) && (y || pr_wait(b, pb, err));
+  return (x || pr_wait_on(a, pa, err)) && (y || pr_wait_on(b, pb, err));
 }
 
 // One lane of the converged warp.  The issuer's loop runs in the whole warp, on
@@ -578,18 +585,22 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
             mbar_expect_tx(&k_full[k_st], uint32_t(c * bk * D * 2));
           }
           __syncwarp();
-          const int c_n = copies(int(rank));
-          const int row = lane < c_n ? row_of(k0 + int(rank) * Cfg::kKeys + lane * bk) : 0;
-          const uint32_t bar = smem_u32(&k_full[k_st]) & (CG == 2 ? kLeaderMask : 0xffffffffu);
-          for (int c = 0; c < c_n; ++c) {
-            const int r = __shfl_sync(0xffffffffu, row, c);
-            if (elect_one()) {
-#pragma unroll
-              for (int piece = 0; piece < Cfg::kPieces; ++piece)
-                pr_tma<CG>(sk + k_st * Cfg::kK + piece * (Cfg::kKeys * 128) + c * bk * 128, &kmap, r,
-                           it.head * Cfg::kPieces + piece, bar);
-            }
+          const uint32_t bar = smem_u32(&k_full[k_st]) & (CG == 2 ? kLeaderMask : 0xffffffffu), to = sk + k_st * Cfg::kK;
+          const int c_n = copies(int(rank)), row = lane < c_n ? row_of(k0 + int(rank) * Cfg::kKeys + lane * bk) : 0;
+          if (p.whole_k) {
+            const int r = __shfl_sync(0xffffffffu, row, 0);
+            if (c_n && elect_one()) pr_tma<CG>(to, &kmap, r, it.head * Cfg::kPieces, bar);
             __syncwarp();
+          } else {
+            for (int c = 0; c < c_n; ++c) {
+              const int r = __shfl_sync(0xffffffffu, row, c);
+              if (elect_one()) {
+#pragma unroll
+                for (int piece = 0; piece < Cfg::kPieces; ++piece)
+                  pr_tma<CG>(to + piece * (Cfg::kKeys * 128) + c * bk * 128, &kmap, r, it.head * Cfg::kPieces + piece, bar);
+              }
+              __syncwarp();
+            }
           }
           if (++k_st == ST) k_st = 0, k_ph ^= 1u;
         }
@@ -601,16 +612,22 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           const int cv = (n + bv - 1) >> p.box_v;
           if (elect_one()) mbar_expect_tx(&v_full[v_st], uint32_t(cv * bv * Cfg::kPiecesV * 128));
           __syncwarp();
-          const int row = lane < cv ? row_of(k0 + lane * bv) : 0;
-          for (int c = 0; c < cv; ++c) {
-            const int r = __shfl_sync(0xffffffffu, row, c);
-            if (elect_one()) {
-#pragma unroll
-              for (int piece = 0; piece < Cfg::kPiecesV; ++piece)
-                pr_tma<CG>(sv + v_st * Cfg::kK + piece * (PR_KEYS * 128) + c * bv * 128, &vmap, r,
-                           it.head * Cfg::kPieces + int(rank) * Cfg::kPiecesV + piece, smem_u32(&v_full[v_st]));
-            }
+          const int row = lane < cv ? row_of(k0 + lane * bv) : 0, first = it.head * Cfg::kPieces + int(rank) * Cfg::kPiecesV;
+          const uint32_t bar = smem_u32(&v_full[v_st]), to = sv + v_st * Cfg::kK;
+          if (p.whole_v) {
+            const int r = __shfl_sync(0xffffffffu, row, 0);
+            if (elect_one()) pr_tma<CG>(to, &vmap, r, first, bar);
             __syncwarp();
+          } else {
+            for (int c = 0; c < cv; ++c) {
+              const int r = __shfl_sync(0xffffffffu, row, c);
+              if (elect_one()) {
+#pragma unroll
+                for (int piece = 0; piece < Cfg::kPiecesV; ++piece)
+                  pr_tma<CG>(to + piece * (PR_KEYS * 128) + c * bv * 128, &vmap, r, first + piece, bar);
+              }
+              __syncwarp();
+            }
           }
           if (++v_st == ST) v_st = 0, v_ph ^= 1u;
         }
@@ -859,6 +876,13 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         uint32_t s[PR_KEYS];
 #pragma unroll
         for (int c = 0; c < PR_KEYS; c += 32) tm_ld32(sa + c, s + c);
+        // meanwhile: m as the other warpgroup left it at the tile before
+        float prev = -INFINITY;
+        if (u > 0) {
+          ok = ok && pr_wait(&m_pass[w4], (v - 1) & 1u, err);
+          prev = *static_cast<volatile float*>(&s_m[lt]);
+        }
+        __syncwarp();
         tm_wait_ld();
         if constexpr (Cfg::kOwnP) {
           tc_before();
@@ -884,24 +908,17 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         float mt = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
         // a score of +inf makes the row NaN (inf - inf), as a NaN does
         if (mt == INFINITY) mt = __int_as_float(0x7fffffff);
-        // m as the other warpgroup left it at the tile before, and on to the next
-        float now = -INFINITY;
-        if (u > 0) {
-          ok = ok && pr_wait(&m_pass[w4], (v - 1) & 1u, err);
-          __syncwarp();
-          now = s_m[lt];
-        }
-        const bool grew = !(mt <= now) && !((mt - now) * sc <= PR_GROW);  // now = -inf and NaN included
-        const float f = grew ? ex2((now - mt) * sc) : 1.0f;
-        if (grew) now = mt;
+        const bool grew = !(mt <= prev) && !((mt - prev) * sc <= PR_GROW);  // prev = -inf and NaN included
+        const float now = grew ? mt : prev;
         s_m[lt] = now;
         __syncwarp();
         if (lane == 0 && ok) mbar_arrive(&m_pass[w4]);
-        if (now != m) {  // (l is 0 as long as m is -inf)
-          l *= ex2((m - now) * sc);
+        if (__any_sync(0xffffffffu, now != m)) {  // rare: some row's m moved, here or there
+          if (now != m) l *= ex2((m - now) * sc);  // (l is 0 as long as m is -inf)
           m = now;
         }
         if (__any_sync(0xffffffffu, grew) && u > 0) {
+          const float f = grew ? ex2((prev - mt) * sc) : 1.0f;
           // O to the new m, once the product before has landed
           ok = ok && pr_wait(&pv_done[wg ^ 1], ((v - 1) >> 1) & 1u, err);
           __syncwarp();
@@ -915,11 +932,6 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             tm_st16(oa + c, o);
           }
-        }
-        if constexpr (Cfg::kOwnP) {  // the P slot: the product that read it last
-          if (v >= 2) ok = ok && pr_wait(&pv_done[wg], ((v >> 1) - 1) & 1u, err);
-          __syncwarp();
-          tc_after();
         }
         const float ms = m == -INFINITY ? 0.0f : m * sc;
         const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(-ms, -ms);
@@ -940,6 +952,11 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
               }
               sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(e0, e1));
               pk[c >> 1] = HalfOps<T>::pack(e0, e1);
+            }
+            if (Cfg::kOwnP && b == 0) {  // the P slot: the product that read it last
+              if (v >= 2) ok = ok && pr_wait(&pv_done[wg], ((v >> 1) - 1) & 1u, err);
+              __syncwarp();
+              tc_after();
             }
             tm_st16(pa + b / 2, pk);
           }
@@ -1126,12 +1143,14 @@ cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, cudaStream_t st) {
   const int page = 1 << p.b.page_shift;
   const int bk = p.b.table ? std::min(Cfg::kKeys, page) : Cfg::kKeys, bv = p.b.table ? std::min(PR_KEYS, page) : PR_KEYS;
   p.box_k = __builtin_ctz(bk);
+  p.whole_k = bk == Cfg::kKeys, p.whole_v = bv == PR_KEYS;
   p.box_v = __builtin_ctz(bv);
   p.slots = int64_t(kv.slots);
   CUtensorMap km, vm;
-  e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, bk, 1);
+  e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, bk,
+                             p.whole_k ? Cfg::kPieces : 1);
   if (e == cudaSuccess)
-    e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, bv, 1);
+    e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, bv, p.whole_v ? Cfg::kPiecesV : 1);
   if (e != cudaSuccess) return e;
   // every sequence adds at most one tile to those of the rows put together
   constexpr int SPAN = PR_ROWS * Cfg::CG;
