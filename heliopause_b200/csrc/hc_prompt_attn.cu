@@ -60,7 +60,7 @@ struct PrCfg {
   static constexpr int CG = D == 64 ? 1 : 2;              // CTAs per MMA
   static constexpr bool kOwnP = D <= 128;                 // P beside S, not over it
   static constexpr uint32_t kTmemO = D == 256 ? 256 : 384;
-  static constexpr int kThreads = 384;                    // 8 softmax warps, producer, issuer, 2 loaders
+  static constexpr int kThreads = 512;                    // 8 softmax warps; K, V, S, O and item warps, 3 more loaders
   static constexpr int kQ = PR_ROWS * D * 2;              // bytes of Q
   static constexpr int kK = PR_KEYS / CG * D * 2;         // bytes of K and of V per stage in this CTA
   static constexpr int kStages = D == 256 ? 2 : 4;
@@ -71,10 +71,10 @@ struct PrCfg {
   static constexpr int kPiecesV = kPieces / CG;           // of them V pieces in this CTA
   __host__ __device__ static constexpr uint32_t p_col(uint32_t slot) { return kOwnP ? 256 + slot * 64 : slot * 128; }
 };
-// registers per thread: launched with 168, the two softmax warpgroups take 208
-// (a row of 128 scores each) from the third
-constexpr int PR_REGS_SOFTMAX = 208, PR_REGS_OTHER = 88;
-static_assert(2 * PR_REGS_SOFTMAX + PR_REGS_OTHER == 3 * 168, "the split is of what the block was launched with");
+// registers per thread: launched with 128, the two softmax warpgroups take 208
+// (a row of 128 scores each) from the other two
+constexpr int PR_REGS_SOFTMAX = 208, PR_REGS_OTHER = 48;
+static_assert(2 * PR_REGS_SOFTMAX + 2 * PR_REGS_OTHER == 4 * 128, "the split is of what the block was launched with");
 
 struct PrArgs {
   AttnArgs a;
@@ -437,8 +437,9 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   using Cfg = PrCfg<D>;
   constexpr int CG = Cfg::CG, ST = Cfg::kStages, SPAN = PR_ROWS * CG;
   constexpr uint32_t FMT = HalfOps<T>::kMap == CU_TENSOR_MAP_DATA_TYPE_FLOAT16 ? 0u : 1u;
-  constexpr int PRODUCER = 8, ISSUER = 9, SCHEDULER = 10, ISSUER_O = 11;  // (11: a second loader at head_dim 256)
-  constexpr int LOADERS = Cfg::kOwnP ? 1 : 2;
+  // the roles behind the softmax warps 0 .. 7; each is a warp of its own, since
+  // what it does per tile is a chain of dependent steps
+  constexpr int LOAD_K = 8, LOAD_V = 9, ISSUER = 10, ISSUER_O = 11, SCHEDULER = 12, LOADERS = 4;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) uint4 clc_resp;
   __shared__ __align__(8) uint64_t q_first, q_full, q_free, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], v_peer[ST];
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       mbar_init(&p_ready[i], 4 * CG);
       mbar_init(&pv_done[i], 1);
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 11);  // every warp but the scheduler
+      mbar_init(&item_empty[i], 15);  // every warp but the scheduler
     }
     for (int w = 0; w < 4; ++w) {
       mbar_init(&m_pass[w], 1);
@@ -552,17 +553,26 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     __syncwarp();
   };
 
-  if (warp >= PRODUCER) {
+  if (warp >= LOAD_K) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
-  if (warp == PRODUCER) {
-    // ---- K and V tiles, K one ahead of V (its product comes first).  Lane i
-    // looks up the tile's i-th page; one lane issues the copies, with operands
-    // that are uniform in the warp (see elect_one: from a lane each they took
-    // 1900 clocks a tile)
+  if (warp == LOAD_K || warp == LOAD_V) {
+    // ---- K or V tiles.  Lane i looks up the tile's i-th page; one lane issues
+    // the copies, with operands that are uniform in the warp (see elect_one).
+    // In a pair each CTA brings half: of K's keys, and of V's dims.
+    const bool is_k = warp == LOAD_K;
+    const int keys = is_k ? Cfg::kKeys : PR_KEYS, pieces = is_k ? Cfg::kPieces : Cfg::kPiecesV;
+    const int shift = is_k ? p.box_k : p.box_v, box = 1 << shift;  // (divisions would cost as much as a tile's products)
+    const bool whole = is_k ? p.whole_k : p.whole_v;
+    const int off = is_k ? int(rank) * Cfg::kKeys : 0, piece0 = is_k ? 0 : int(rank) * Cfg::kPiecesV;
+    const CUtensorMap* map = is_k ? &kmap : &vmap;
+    const uint32_t stages = is_k ? sk : sv;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = is_k ? k_empty : v_empty;
+    // K's halves both report to the pair's first CTA, whose thread uses them
+    const bool mine = !is_k || rank == 0;
     PrItem it;
-    const int bk = 1 << p.box_k, bv = 1 << p.box_v;  // (divisions here would cost as much as a tile's products)
-    int k_st = 0, v_st = 0;
-    uint32_t k_ph = 1, v_ph = 1;  // parity of the stage's last release; the first use waits for none
+    int st = 0;
+    uint32_t ph = 1;  // parity of the stage's last release; the first use waits for none
     for (int n_it = 0; next_item(n_it, &it); ++n_it) {
       const PrGeom g = pr_geom(it, group, window, SPAN);
       const auto row_of = [&](int key) {
@@ -572,75 +582,40 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         if (!in && err) atomicExch(err, DEVICE_ERR_PAGE);
         return in ? int((int64_t(page) << p.b.page_shift) + (key & ((1 << p.b.page_shift) - 1))) : int(p.slots);
       };
-      for (int i = 0; i <= g.units && ok && g.units > 0; ++i) {
-        if (i < g.units) {  // K: this CTA's keys, every piece
-          const int k0 = g.key0 + i * PR_KEYS, n = min(PR_KEYS, g.key_hi - k0);
-          ok = pr_wait(&k_empty[k_st], k_ph, err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const auto copies = [&](int r) { return (min(Cfg::kKeys, max(0, n - r * Cfg::kKeys)) + bk - 1) >> p.box_k; };
-          if (rank == 0 && elect_one()) {
-            int c = copies(0);
-            if (CG == 2) c += copies(1);
-            mbar_expect_tx(&k_full[k_st], uint32_t(c * bk * D * 2));
-          }
+      const int first = it.head * Cfg::kPieces + piece0;
+      for (int k0 = g.key0, i = 0; i < g.units; ++i, k0 += PR_KEYS) {
+        const int n = min(PR_KEYS, g.key_hi - k0);
+        const auto copies = [&](int from) { return (min(keys, max(0, n - from)) + box - 1) >> shift; };
+        const int c_n = copies(off);
+        const int row = lane < c_n ? row_of(k0 + off + lane * box) : 0;
+        ok = ok && pr_wait(&empty[st], ph, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&full[st]) & (CG == 2 && is_k ? kLeaderMask : 0xffffffffu), to = stages + st * Cfg::kK;
+        if (mine && elect_one())
+          mbar_expect_tx(&full[st], uint32_t((is_k && CG == 2 ? c_n + copies(Cfg::kKeys) : c_n) * box * pieces * 128));
+        __syncwarp();
+        if (whole) {
+          const int r = __shfl_sync(0xffffffffu, row, 0);
+          if (c_n && elect_one()) pr_tma<CG>(to, map, r, first, bar);
           __syncwarp();
-          const uint32_t bar = smem_u32(&k_full[k_st]) & (CG == 2 ? kLeaderMask : 0xffffffffu), to = sk + k_st * Cfg::kK;
-          const int c_n = copies(int(rank)), row = lane < c_n ? row_of(k0 + int(rank) * Cfg::kKeys + lane * bk) : 0;
-          if (p.whole_k) {
-            const int r = __shfl_sync(0xffffffffu, row, 0);
-            if (c_n && elect_one()) pr_tma<CG>(to, &kmap, r, it.head * Cfg::kPieces, bar);
+        } else {
+          for (int c = 0; c < c_n; ++c) {
+            const int r = __shfl_sync(0xffffffffu, row, c);
+            if (elect_one())
+              for (int piece = 0; piece < pieces; ++piece)
+                pr_tma<CG>(to + piece * (keys * 128) + c * box * 128, map, r, first + piece, bar);
             __syncwarp();
-          } else {
-            for (int c = 0; c < c_n; ++c) {
-              const int r = __shfl_sync(0xffffffffu, row, c);
-              if (elect_one()) {
-#pragma unroll
-                for (int piece = 0; piece < Cfg::kPieces; ++piece)
-                  pr_tma<CG>(to + piece * (Cfg::kKeys * 128) + c * bk * 128, &kmap, r, it.head * Cfg::kPieces + piece, bar);
-              }
-              __syncwarp();
-            }
           }
-          if (++k_st == ST) k_st = 0, k_ph ^= 1u;
         }
-        if (i > 0) {  // V: every key, this CTA's pieces
-          const int k0 = g.key0 + (i - 1) * PR_KEYS, n = min(PR_KEYS, g.key_hi - k0);
-          ok = pr_wait(&v_empty[v_st], v_ph, err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int cv = (n + bv - 1) >> p.box_v;
-          if (elect_one()) mbar_expect_tx(&v_full[v_st], uint32_t(cv * bv * Cfg::kPiecesV * 128));
-          __syncwarp();
-          const int row = lane < cv ? row_of(k0 + lane * bv) : 0, first = it.head * Cfg::kPieces + int(rank) * Cfg::kPiecesV;
-          const uint32_t bar = smem_u32(&v_full[v_st]), to = sv + v_st * Cfg::kK;
-          if (p.whole_v) {
-            const int r = __shfl_sync(0xffffffffu, row, 0);
-            if (elect_one()) pr_tma<CG>(to, &vmap, r, first, bar);
-            __syncwarp();
-          } else {
-            for (int c = 0; c < cv; ++c) {
-              const int r = __shfl_sync(0xffffffffu, row, c);
-              if (elect_one()) {
-#pragma unroll
-                for (int piece = 0; piece < Cfg::kPiecesV; ++piece)
-                  pr_tma<CG>(to + piece * (PR_KEYS * 128) + c * bv * 128, &vmap, r, first + piece, bar);
-              }
-              __syncwarp();
-            }
-          }
-          if (++v_st == ST) v_st = 0, v_ph ^= 1u;
-        }
+        if (++st == ST) st = 0, ph ^= 1u;
       }
       if (!ok) break;
     }
     // after a timeout: the copies that nobody else waits for
-    if (!ok)
-      for (int i = 0; i < ST; ++i) {
-        if (rank == 0) pr_wait(&k_full[i], k_ph, nullptr);
-        pr_wait(&v_full[i], v_ph, nullptr);
-      }
-  } else if (warp == ISSUER || (Cfg::kOwnP && warp == ISSUER_O)) {
+    if (!ok && mine)
+      for (int i = 0; i < ST; ++i) pr_wait(&full[i], ph, nullptr);
+  } else if (warp == ISSUER || warp == ISSUER_O) {
     // ---- the products, issued by one thread of the pair's first CTA.  What
     // an issuer does between a barrier and its product is on every tile's path
     // (all its waits and descriptors took over 1000 clocks a tile, as
@@ -692,7 +667,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     PrItem it;
     for (int n_it = 0; next_item(n_it, &it); ++n_it) {
       const PrGeom g = pr_geom(it, group, window, SPAN);
-      if (g.units == 0) continue;
+      if (g.units == 0 || (warp == ISSUER_O && !Cfg::kOwnP)) continue;
       if (rank != 0) {  // the second CTA reports its half of every V tile
         if (warp == ISSUER)
           for (int i = 0; i < g.units; ++i) {
@@ -759,7 +734,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     int s0 = 0, before = 0;  // items of the sequences before s0
     int x = int(blockIdx.x) / CG;
     int nq = 0;
-    const int l64 = t - 32 * SCHEDULER;
+    const int loader = t - 32 * SCHEDULER;
     for (int n_it = 0; ok; ++n_it) {
       PrItem it;
       it.seq = -1;
@@ -831,7 +806,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           if (nq > 0) ok = pr_wait(&q_free, uint32_t(nq - 1) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          load_q(it, g, l64, 32 * LOADERS);
+          load_q(it, g, loader, 32 * LOADERS);
         }
         if (lane == 0) arrive_leader<CG>(&q_full);
         ++nq;
