@@ -254,18 +254,25 @@ __device__ __forceinline__ void sync_all() {
 }
 __device__ __forceinline__ bool pr_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                : "=r"(ok)
                : "r"(smem_u32(bar)), "r"(parity)
                : "memory");
   return ok != 0;
 }
-// The rest of a wait, bounded in time.
+// The rest of a wait, bounded in time.  The hint lets the hardware suspend the
+// warp until the phase is complete: without it the waiting warps of a block took a
+// quarter of the issue slots.
+constexpr uint32_t PR_SLEEP_NS = 1000000;
 __device__ __forceinline__ bool pr_wait_on(uint64_t* bar, uint32_t parity, int* err) {
   unsigned long long t0 = 0;
   for (int it = 0;; ++it) {
-    if (pr_try(bar, parity)) return true;
-    if (it & 15) continue;
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity), "r"(PR_SLEEP_NS)
+                 : "memory");
+    if (ok) return true;
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     if (it == 0) {

@@ -346,7 +346,7 @@ int hpc_prompt_attention(const void *d_q, size_t q_stride, const void *d_k, size
  * logit l of a row, in f64 and rounded once to f32:
  *   seen in the row's history:  x = l > 0 ? l / repetition : l * repetition
  *   c > 0 times in its output:  x = x - frequency * c - presence
- *   the row's biases of i, in list order:  x = x + bias
+ *   the row's biases of i, added up in list order:  x = x + sum
  *   its mask bit is 0:          x = -inf
  * History of row r: d_history[starts[r] .. starts[r + 1]), the first
  * prompt_lens[r] entries its prompt (seen, not counted; NULL: none), the rest

