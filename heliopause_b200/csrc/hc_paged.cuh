@@ -93,6 +93,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// One lane of the converged warp.  Code that issues TMA copies or MMAs runs in
+// the whole warp, on values that are the same in every lane, and only the
+// instruction itself stands behind this: inside a branch on the lane number
+// the compiler passes each one's operands lane by lane (about 80 clocks per
+// instruction).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ void pdl_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_next() { asm volatile("griddepcontrol.launch_dependents;"); }
 

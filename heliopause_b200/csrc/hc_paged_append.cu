@@ -25,7 +25,7 @@
 namespace hc {
 namespace {
 
-constexpr int AP_MAX_WARPS = 16;
+constexpr int AP_MAX_WARPS = 8;
 
 struct AppendArgs {
   const void* src[3];     // q (or nullptr), k, v
@@ -94,7 +94,7 @@ __device__ __forceinline__ int find_seq(const int32_t* starts, int seqs, int t, 
   return lo;
 }
 
-template <class TIn, class T, int E>
+template <class TIn, class T, int E, int PER>
 __global__ void __launch_bounds__(32 * AP_MAX_WARPS) hc_paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int D = 32 * E;
   __shared__ float2 turn[D / 2];  // (cos, sin)
@@ -110,8 +110,10 @@ __global__ void __launch_bounds__(32 * AP_MAX_WARPS) hc_paged_append_kernel(cons
   pdl_launch_next();
   pdl_wait_prior();
   int part, hh;
-  float x[E];
-  load_row<TIn, E>(row_of(min(warp, total - 1), &part, &hh), x);
+  float xs[PER][E];  // this warp's first PER heads
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (warp + i * warps < total) load_row<TIn, E>(row_of(warp + i * warps, &part, &hh), xs[i]);
   if (warp == 0) {
     const int s = find_seq(a.b.starts, a.b.seqs, t, lane);
     if (lane == 0) {
@@ -142,9 +144,8 @@ __global__ void __launch_bounds__(32 * AP_MAX_WARPS) hc_paged_append_kernel(cons
     __syncthreads();
   }
   const int64_t slot = (int64_t(s_page) << a.b.page_shift) + (pos & ((1 << a.b.page_shift) - 1));
-  for (int h = warp; h < total; h += warps) {
-    const TIn* src = row_of(h, &part, &hh);
-    if (h != warp) load_row<TIn, E>(src, x);
+  const auto head = [&](int h, float(&x)[E]) {
+    row_of(h, &part, &hh);
     if (a.norm[part]) {
       float ss = 0.0f;
 #pragma unroll
@@ -178,19 +179,35 @@ __global__ void __launch_bounds__(32 * AP_MAX_WARPS) hc_paged_append_kernel(cons
     T* dst = part == 0 ? static_cast<T*>(a.q_out) + (int64_t(t) * hq + hh) * D
                        : static_cast<T*>(a.cache[part - 1]) + (slot * hk + hh) * D;
     store_row<T, E>(dst + lane * E, x);
+  };
+  // PER rows in flight: a row's successor is loaded before its partner is used
+  for (int h = warp; h < total; h += PER * warps) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (h + i * warps >= total) break;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = xs[i][e];
+      const int after = h + (PER + i) * warps;
+      if (after < total) load_row<TIn, E>(row_of(after, &part, &hh), xs[i]);
+      head(h + i * warps, x);
+    }
   }
+}
+
+template <class TIn, class T, int E>
+cudaError_t launch_append_e(const AppendArgs& a, cudaStream_t st) {
+  const int total = a.heads[0] + 2 * a.heads[1];
+  const int per = (total + AP_MAX_WARPS - 1) / AP_MAX_WARPS;  // heads a warp takes, evenly
+  const dim3 grid(unsigned(a.b.rows)), block(unsigned(32 * ((total + per - 1) / per)));
+  return per == 1 ? launch_pdl(hc_paged_append_kernel<TIn, T, E, 1>, grid, block, 0, st, a)
+                  : launch_pdl(hc_paged_append_kernel<TIn, T, E, 2>, grid, block, 0, st, a);
 }
 
 template <class TIn, class T>
 cudaError_t launch_append(const AppendArgs& a, int dim, cudaStream_t st) {
-  const int total = a.heads[0] + 2 * a.heads[1];
-  const int per = (total + AP_MAX_WARPS - 1) / AP_MAX_WARPS;  // heads a warp takes, evenly
-  const dim3 grid(unsigned(a.b.rows)), block(unsigned(32 * ((total + per - 1) / per)));
-  switch (dim) {
-    case 64: return launch_pdl(hc_paged_append_kernel<TIn, T, 2>, grid, block, 0, st, a);
-    case 128: return launch_pdl(hc_paged_append_kernel<TIn, T, 4>, grid, block, 0, st, a);
-    default: return launch_pdl(hc_paged_append_kernel<TIn, T, 8>, grid, block, 0, st, a);
-  }
+  return dim == 64 ? launch_append_e<TIn, T, 2>(a, st) : dim == 128 ? launch_append_e<TIn, T, 4>(a, st)
+                                                                    : launch_append_e<TIn, T, 8>(a, st);
 }
 
 }  // namespace

@@ -243,8 +243,9 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
   int it = 0;  // K and V tiles so far: slot it % kSlots, phase it / kSlots
   bool ok = true;
   if (warp == AR_WARPS) {
-    // ---- producer: lane i copies the tile's i-th page
-    const int box = p.box_rows, ppt = AR_TILE / box;
+    // ---- producer: lane i looks up the tile's i-th page; one lane issues the
+    // copies, with operands that are uniform in the warp (elect_one)
+    const int box = p.box_rows, box_shift = __ffs(box) - 1, ppt = AR_TILE >> box_shift;
     while (w.u < w.end && ok) {
       bool bad;
       const SeqSpan q = seq_span(p.b, w.s, &bad);
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
           for (; w.tile < st.count && w.u < w.end && ok; ++w.tile, ++w.u) {
             const int k0 = (st.first + w.tile) * AR_TILE;
             if (k0 + AR_TILE <= sp.lo || k0 >= sp.hi) continue;
-            const int copies = (min(AR_TILE, q.len - k0) + box - 1) / box;
+            const int copies = (min(AR_TILE, q.len - k0) + box - 1) >> box_shift;
             int row = 0;
             if (lane < ppt && lane < copies) {
               if (p.b.table) {
@@ -274,11 +275,15 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
               if (ph > 0 && !mbar_wait_parity_sleep(&empty[slot], uint32_t(ph - 1) & 1u, p.a.err)) ok = false;
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
-              if (lane == 0) mbar_expect_tx(&full[slot], uint32_t(copies * box * D * 2));
+              if (elect_one()) mbar_expect_tx(&full[slot], uint32_t(copies * box * D * 2));
               __syncwarp();
-              if (lane < copies)
-                tma_load_3d(base + slot * Cfg::kSlot + lane * box * D * 2, kv ? &vmap : &kmap, 0, row,
-                            w.head * (D / 64), smem_u32(&full[slot]));
+              for (int c = 0; c < copies; ++c) {
+                const int r = __shfl_sync(0xffffffffu, row, c);
+                if (elect_one())
+                  tma_load_3d(base + slot * Cfg::kSlot + c * box * D * 2, kv ? &vmap : &kmap, 0, r, w.head * (D / 64),
+                              smem_u32(&full[slot]));
+                __syncwarp();
+              }
             }
           }
         }
@@ -575,12 +580,19 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
 }
 
 // Joins the partials of the item whose first tile CTA blockIdx.x held, one
-// row per block: the maximum of all, then the sums in CTA order.
+// row per block: the maximum of all, then the sums, by groups of D / 4 threads
+// that take every GROUPS-th partial each (one long sequence leaves a partial on
+// every SM), added up in the groups' order.
+constexpr int AJ_THREADS = 256, AJ_PARTS = 512;
 template <class T, int D, int NB>
-__global__ void __launch_bounds__(D / 2) hc_attn_join_kernel(const __grid_constant__ RowsArgs p, int grid) {
-  constexpr int R = 8 * NB, TH = D / 2;
-  __shared__ float s_max[TH / 32], s_f[TH];
-  __shared__ int s_part[TH];
+__global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_constant__ RowsArgs p, int grid) {
+  constexpr int R = 8 * NB, LANES = D / 4, GROUPS = AJ_THREADS / LANES;
+  __shared__ int s_part[AJ_PARTS];
+  __shared__ float2 s_ml[AJ_PARTS];
+  __shared__ int s_n;
+  __shared__ float s_max[AJ_THREADS / 32];
+  __shared__ float4 s_o[GROUPS][LANES];
+  __shared__ float s_sum[GROUPS];
   const int c0 = int(blockIdx.x), r = int(blockIdx.y), t = int(threadIdx.x);
   pdl_wait_prior();
   const JoinRec rec = p.w.rec[c0];
@@ -590,53 +602,63 @@ __global__ void __launch_bounds__(D / 2) hc_attn_join_kernel(const __grid_consta
   const int group = p.a.heads / p.a.kv_heads;
   const int r0 = rec.block * R;
   if (r >= min(R, q.n * group - r0)) return;
-  const auto part_of = [&](int c) { return c == c0 ? 2 * c + 1 : 2 * c; };
-  const auto held = [&](int c) { return cta_begin(rec.total, c, grid) < cta_begin(rec.total, c + 1, grid); };
+  // the partials, in CTA order; a CTA that held no tile left none
+  if (t < 32) {
+    int n = 0;
+    for (int b = c0; b <= rec.last; b += 32) {
+      const int c = b + t;
+      const bool has = c <= rec.last && cta_begin(rec.total, c, grid) < cta_begin(rec.total, c + 1, grid);
+      const unsigned m = __ballot_sync(0xffffffffu, has);
+      if (has) s_part[n + __popc(m & ((1u << t) - 1u))] = c == c0 ? 2 * c + 1 : 2 * c;
+      n += __popc(m);
+    }
+    if (t == 0) s_n = n;
+  }
+  __syncthreads();
+  const int n = s_n;
   float mx = -INFINITY;
-  for (int c = c0 + t; c <= rec.last; c += TH)
-    if (held(c)) mx = fmaxf(mx, p.w.ml[part_of(c) * R + r].x);
+  for (int i = t; i < n; i += AJ_THREADS) {
+    const float2 v = p.w.ml[s_part[i] * R + r];
+    s_ml[i] = v;
+    mx = fmaxf(mx, v.x);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if ((t & 31) == 0) s_max[t >> 5] = mx;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < TH / 32; ++i) mx = fmaxf(mx, s_max[i]);
+  for (int i = 0; i < AJ_THREADS / 32; ++i) mx = fmaxf(mx, s_max[i]);
   const float ms = mx == -INFINITY ? 0.0f : mx;
-  float sum = 0.0f, x = 0.0f, y = 0.0f;
-  for (int b = c0; b <= rec.last; b += TH) {
-    __syncthreads();
-    const int c = b + t;
-    if (c <= rec.last) {
-      float f = 0.0f;
-      int part = -1;
-      if (held(c)) {
-        part = part_of(c);
-        const float2 v = p.w.ml[part * R + r];
-        f = ex2(v.x - ms);
-        // summed below in CTA order by every thread alike
-      }
-      s_f[t] = f;
-      s_part[t] = part;
-    }
-    __syncthreads();
-    const int n = min(TH, rec.last - b + 1);
+  const int g = t / LANES, d = t % LANES * 4;
+  float sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const int part = s_part[i];
-      if (part < 0) continue;
-      const float f = s_f[i];
-      const float2 v = *reinterpret_cast<const float2*>(p.w.o + (int64_t(part) * R + r) * D + 2 * t);
-      sum += f * p.w.ml[part * R + r].y;
-      x += f * v.x;
-      y += f * v.y;
-    }
+  for (int i = g; i < n; i += GROUPS) {
+    const float f = ex2(s_ml[i].x - ms);
+    const float4 v = *reinterpret_cast<const float4*>(p.w.o + (int64_t(s_part[i]) * R + r) * D + d);
+    sum += f * s_ml[i].y;
+    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  }
+  s_o[g][t % LANES] = o;
+  if (t % LANES == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (g != 0) return;
+  sum = 0.0f;
+  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float4 v = s_o[i][t];
+    sum += s_sum[i];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   const int64_t row = int64_t(q.row0 + (r0 + r) / group) * p.a.heads + rec.head * group + (r0 + r) % group;
   if (p.a.out_f32)
-    *reinterpret_cast<float2*>(static_cast<float*>(p.a.out) + row * D + 2 * t) = make_float2(x * inv, y * inv);
+    *reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + row * D + d) =
+        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   else
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.a.out) + row * D + 2 * t) = HalfOps<T>::pack(x * inv, y * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + row * D + d) =
+        make_uint2(HalfOps<T>::pack(o.x * inv, o.y * inv), HalfOps<T>::pack(o.z * inv, o.w * inv));
   if (t == 0 && p.a.lse) p.a.lse[row] = sum == 0.0f ? -INFINITY : LN2 * (mx + log2f(sum));
 }
 
@@ -675,7 +697,8 @@ cudaError_t launch_rows(RowsArgs& p, const KvSource& kv, void* workspace, cudaSt
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(grid), dim3(AR_THREADS), Cfg::kSmem, st, km, vm, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(hc_attn_join_kernel<T, D, NB>, dim3(grid, 8 * NB), dim3(D / 2), 0, st, p, grid);
+  static_assert(3 * kMaxSms <= AJ_PARTS, "one partial per CTA at most");
+  return launch_pdl(hc_attn_join_kernel<T, D, NB>, dim3(grid, 8 * NB), dim3(AJ_THREADS), 0, st, p, grid);
 }
 
 template <class T, int D>

@@ -295,16 +295,6 @@ __device__ __forceinline__ bool pr_wait2(uint64_t* a, uint32_t pa, uint64_t* b, 
   return (x || pr_wait_on(a, pa, err)) && (y || pr_wait_on(b, pb, err));
 }
 
-// One lane of the converged warp.  The issuer's loop runs in the whole warp, on
-// values that are the same in every lane, and only the instructions that one
-// thread has to issue stand behind this: inside a branch on the lane number
-// the compiler passes each MMA's operands one by one (about 80 clocks per MMA).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
-  return r != 0;
-}
-
 // ---- the launch's next item (clusterlaunchcontrol) ------------------------------
 
 // Asks for a cluster of this grid that has not started; the answer (16 bytes)

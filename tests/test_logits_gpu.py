@@ -150,6 +150,30 @@ def test_ties_across_chunks_and_many_equal_values():
     _same(g.integers(-1000, 1000, (4, 50_000)).astype(np.float32), 64)
 
 
+def test_ties_between_touched_and_untouched_tokens():
+    # integer logits: penalties and biases put touched tokens on the values of
+    # untouched ones, behind and before them
+    g = np.random.default_rng(21)
+    rows, vocab = 3, 40_000
+    x = g.integers(-4, 5, (rows, vocab)).astype(np.float32)
+    x[:, g.choice(vocab, 300, replace=False)] = 9.0
+    hs = [np.concatenate([g.integers(0, vocab, 500), np.nonzero(x[r] == 9)[0][-60:]]) for r in range(rows)]
+    bias = [[(int(i), 5.0) for i in np.concatenate([g.choice(np.nonzero(x[r] == 4)[0], 100), [vocab - 1, 0]])] for r in range(rows)]
+    for k in (5, 64):
+        _same(x, k, hist=hs, freq=np.ones(rows, np.float32), bias=bias)
+        _same(x, k, hist=hs, freq=-np.ones(rows, np.float32), bias=bias, allowed=g.random((rows, vocab)) < 0.5)
+
+
+def test_long_histories_and_many_biases():
+    # more tokens than a count's bits, more biases and listed tokens than the lists hold
+    g = np.random.default_rng(22)
+    x = (g.standard_normal((2, 70_000)) * 2).astype(np.float32)
+    hs = [np.full(20_000, 77), g.integers(0, 12_000, 30_000)]
+    bias = [[(int(i), float(v)) for i, v in zip(g.integers(0, 9000, 1500), g.standard_normal(1500))], [(5, 1.5)] * 700]
+    _same(x, 64, hist=hs, prompt=np.array([10, 5000]), rep=np.array([1.1, 0.9], np.float32),
+          freq=np.array([-0.001, 0.25], np.float32), pres=np.array([0.5, -0.5], np.float32), bias=bias)
+
+
 def test_starts_outside_the_lists_are_bounded():
     x = torch.randn((2, 500), device="cuda")
     h = torch.arange(10, dtype=torch.int32, device="cuda")
