@@ -348,35 +348,45 @@ def device_error() -> None:
 _DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _raw_stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _check_i32(name: str, device: torch.device, *tensors: torch.Tensor) -> None:
+def _check_i32(name: str, dev: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
             raise CudaKernelError(ERR_ARG, f"{name}: starts, lengths and page tables are contiguous int32 tensors on "
-                                           f"{device}")
+                                           f"cuda:{dev}")
 
 
-def _rows3(name: str, t: torch.Tensor, device: torch.device, heads: int, dim: int) -> torch.Tensor:
-    """[rows][heads][dim] on `device`, heads and elements contiguous within a row."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device:
-        raise CudaKernelError(ERR_SHAPE, f"{name}: [rows][{heads}][{dim}] on {device}, not {tuple(t.shape)} on {t.device}")
+def _rows3(name: str, t: torch.Tensor, dev: int, shape: tuple) -> tuple[torch.Tensor, int]:
+    """[rows][heads][dim] on the device, heads and elements contiguous within a row; and its row stride."""
+    if t.shape != shape or t.get_device() != dev:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {shape} on cuda:{dev}, not {tuple(t.shape)} on {t.device}")
+    rows, heads, dim = shape
     st = t.stride()
     if st[2] != 1 or (st[1] != dim and heads > 1) or st[0] % 8 or st[0] < heads * dim or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.stride(0) != heads * dim:  # a single row keeps any stride
-            t = t.as_strided(t.shape, (heads * dim, dim, 1))
-    return t
+        return t.clone(memory_format=torch.contiguous_format), heads * dim
+    return t, st[0]
 
 
 def _check_cache(name: str, key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
     if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
         raise CudaKernelError(ERR_SHAPE, f"{name}: key and value caches are [pages][page_size][kv_heads][head_dim]")
-    if not (key_cache.is_cuda and key_cache.device == value_cache.device and key_cache.is_contiguous()
+    if not (key_cache.is_cuda and key_cache.get_device() == value_cache.get_device() and key_cache.is_contiguous()
             and value_cache.is_contiguous()):
         raise CudaKernelError(ERR_ARG, f"{name}: the caches are contiguous tensors on one device")
+
+
+def _check_batch(name: str, dev: int, page_table: torch.Tensor, query_starts: torch.Tensor,
+                 kv_lens: torch.Tensor) -> tuple[int, int]:
+    """Sequences and the page table's width."""
+    _check_i32(name, dev, page_table, query_starts, kv_lens)
+    seqs, table = kv_lens.numel(), page_table.shape
+    if len(table) != 2 or table[0] != seqs or query_starts.numel() != seqs + 1:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {seqs} sequences, a table of {tuple(table)}, "
+                                         f"{query_starts.numel()} starts")
+    return seqs, table[1]
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -396,67 +406,70 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, v
     page_table[s][j // page_size].  Rows behind the last sequence are left."""
     name = "pagedKvAppend"
     _check_cache(name, key_cache, value_cache)
+    dev, dt = key_cache.get_device(), key_cache.dtype
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return paged_kv_append(k, v, key_cache, value_cache, page_table, query_starts, kv_lens, q=q,
+                                   inv_freq=inv_freq, q_norm=q_norm, k_norm=k_norm, norm_v=norm_v, eps=eps, q_out=q_out)
     pages, page_size, kv_heads, dim = key_cache.shape
-    dev, dt = key_cache.device, key_cache.dtype
-    _check_i32(name, dev, page_table, query_starts, kv_lens)
-    seqs = kv_lens.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or query_starts.numel() != seqs + 1:
-        raise CudaKernelError(ERR_SHAPE, f"{name}: {seqs} sequences, a table of {tuple(page_table.shape)}, "
-                                         f"{query_starts.numel()} starts")
-    k = _rows3(name, k, dev, kv_heads, dim)
-    v = _rows3(name, v, dev, kv_heads, dim)
+    seqs, width = _check_batch(name, dev, page_table, query_starts, kv_lens)
+    xt = k.dtype
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != xt:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: keys of {tuple(k.shape)} {xt}, values of {tuple(v.shape)} {v.dtype}")
+    if dt not in _DTYPE_IDS or xt not in _DTYPE_IDS:
+        raise CudaKernelError(ERR_TYPE, f"{name}: {xt} into a cache of {dt}")
     rows, heads = k.shape[0], kv_heads
-    if v.shape[0] != rows or v.dtype != k.dtype:
-        raise CudaKernelError(ERR_SHAPE, f"{name}: keys and values differ in rows or type")
-    if dt not in _DTYPE_IDS or k.dtype not in _DTYPE_IDS:
-        raise CudaKernelError(ERR_TYPE, f"{name}: {k.dtype} into a cache of {dt}")
-    qp = qs = op = 0
+    shape = (rows, kv_heads, dim)
+    k, ks = _rows3(name, k, dev, shape)
+    v, vs = _rows3(name, v, dev, shape)
+    qp = op = None
+    qs = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != rows or q.dtype != k.dtype:
+        if q.dim() != 3 or q.shape[0] != rows or q.dtype != xt:
             raise CudaKernelError(ERR_SHAPE, f"{name}: queries and keys differ in rows or type")
         heads = q.shape[1]
-        q = _rows3(name, q, dev, heads, dim)
+        shape = (rows, heads, dim)
+        q, qs = _rows3(name, q, dev, shape)
         if q_out is None:
-            q_out = torch.empty((rows, heads, dim), dtype=dt, device=dev)
-        elif q_out.shape != q.shape or q_out.dtype != dt or q_out.device != dev or not q_out.is_contiguous():
-            raise CudaKernelError(ERR_SHAPE, f"{name}: q_out is contiguous {tuple(q.shape)} of {dt}")
-        qp, qs, op = q.data_ptr(), q.stride(0), q_out.data_ptr()
-    half = 0
+            q_out = key_cache.new_empty(shape)
+        elif q_out.shape != shape or q_out.dtype != dt or q_out.get_device() != dev or not q_out.is_contiguous():
+            raise CudaKernelError(ERR_SHAPE, f"{name}: q_out is contiguous {shape} of {dt}")
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    fp, half = None, 0
     if inv_freq is not None:
-        if inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous():
-            raise CudaKernelError(ERR_ARG, f"{name}: inv_freq is a contiguous float64 tensor on {dev}")
+        if inv_freq.dtype is not torch.float64 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+            raise CudaKernelError(ERR_ARG, f"{name}: inv_freq is a contiguous float64 tensor on cuda:{dev}")
         half = inv_freq.numel()
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != dim or w.device != dev or not w.is_contiguous()):
-            raise CudaKernelError(ERR_ARG, f"{name}: norm weights are {dim} contiguous float32 values on {dev}")
-    with _on_device(dev):
-        code = _lib.lib().hpc_paged_kv_append(
-            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), qp, qs, _DTYPE_IDS[k.dtype], rows, heads, kv_heads, dim,
-            inv_freq.data_ptr() if half else None, half, q_norm.data_ptr() if q_norm is not None else None,
-            k_norm.data_ptr() if k_norm is not None else None, int(norm_v), eps, key_cache.data_ptr(),
-            value_cache.data_ptr(), _DTYPE_IDS[dt], pages, page_size, page_table.data_ptr(), page_table.shape[1],
-            query_starts.data_ptr(), kv_lens.data_ptr(), seqs, op, _raw_stream(dev))
+        fp = inv_freq.data_ptr() if half else None
+    norms = [None, None]
+    for i, w in enumerate((q_norm, k_norm)):
+        if w is not None:
+            if w.dtype is not torch.float32 or w.numel() != dim or w.get_device() != dev or not w.is_contiguous():
+                raise CudaKernelError(ERR_ARG, f"{name}: norm weights are {dim} contiguous float32 values on cuda:{dev}")
+            norms[i] = w.data_ptr()
+    code = _lib.lib().hpc_paged_kv_append(
+        k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, _DTYPE_IDS[xt], rows, heads, kv_heads, dim, fp, half, norms[0],
+        norms[1], norm_v, eps, key_cache.data_ptr(), value_cache.data_ptr(), _DTYPE_IDS[dt], pages, page_size,
+        page_table.data_ptr(), width, query_starts.data_ptr(), kv_lens.data_ptr(), seqs, op, _raw_stream(dev))
     if code:
         assert_cuda_ok(code, name)
     return q_out if q is not None else None
 
 
-class _on_device:
-    """Makes `device` current for a call when another one is."""
-    __slots__ = ("index", "back")
+class _workspace:
+    """Device memory for the length of one call on the current stream: the
+    allocator hands a freed block on in stream order, as with a tensor, at a
+    third of a tensor's cost (0.5 us against 1.5)."""
+    __slots__ = ("ptr",)
 
-    def __init__(self, device: torch.device):
-        self.index = device.index
+    def __init__(self, nbytes: int, stream: int):
+        self.ptr = torch._C._cuda_cudaCachingAllocator_raw_alloc(nbytes, stream)
 
-    def __enter__(self):
-        cur = torch._C._cuda_getDevice()
-        self.back = cur if cur != self.index else -1
-        if self.back >= 0:
-            torch.cuda.set_device(self.index)
+    def __enter__(self) -> int:
+        return self.ptr
 
     def __exit__(self, *exc):
-        if self.back >= 0:
-            torch.cuda.set_device(self.back)
+        torch._C._cuda_cudaCachingAllocator_raw_delete(self.ptr)
 
 
 @functools.lru_cache(maxsize=None)
@@ -466,15 +479,15 @@ def _attention_workspace(heads: int, kv_heads: int, dim: int) -> int:
     return n.value
 
 
-def _attention_out(name, q, out, out_dtype, return_lse):
+def _attention_out(name: str, dev: int, shape: tuple, q: torch.Tensor, out, out_dtype, return_lse):
     dt = out.dtype if out is not None else out_dtype or q.dtype
-    if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
-    elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
-        raise CudaKernelError(ERR_SHAPE, f"{name}: out is contiguous {tuple(q.shape)} on {q.device}")
     if dt not in _DTYPE_IDS:
         raise CudaKernelError(ERR_TYPE, f"{name}: output of {dt}")
-    lse = torch.full(q.shape[:2], -torch.inf, dtype=torch.float32, device=q.device) if return_lse else None
+    if out is None:
+        out = q.new_empty(shape) if dt is q.dtype else q.new_empty(shape, dtype=dt)
+    elif out.shape != shape or out.get_device() != dev or not out.is_contiguous():
+        raise CudaKernelError(ERR_SHAPE, f"{name}: out is contiguous {shape} on cuda:{dev}")
+    lse = torch.full(shape[:2], -torch.inf, dtype=torch.float32, device=q.device) if return_lse else None
     return out, lse
 
 
@@ -490,28 +503,29 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     return_lse)."""
     name = "pagedAttention"
     _check_cache(name, key_cache, value_cache)
+    dev, dt = key_cache.get_device(), key_cache.dtype
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return paged_attention(q, key_cache, value_cache, page_table, query_starts, kv_lens,
+                                   max_query_len=max_query_len, scale=scale, window=window, out=out,
+                                   out_dtype=out_dtype, return_lse=return_lse)
     pages, page_size, kv_heads, dim = key_cache.shape
-    dev, dt = key_cache.device, key_cache.dtype
-    _check_i32(name, dev, page_table, query_starts, kv_lens)
-    seqs = kv_lens.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or query_starts.numel() != seqs + 1:
-        raise CudaKernelError(ERR_SHAPE, f"{name}: {seqs} sequences, a table of {tuple(page_table.shape)}, "
-                                         f"{query_starts.numel()} starts")
+    seqs, width = _check_batch(name, dev, page_table, query_starts, kv_lens)
     if q.dim() != 3 or q.dtype != dt:
         raise CudaKernelError(ERR_TYPE, f"{name}: queries of {q.dtype} over a cache of {dt}")
-    rows, heads = q.shape[:2]
-    q = _rows3(name, q, dev, heads, dim)
+    rows, heads, _ = q.shape
+    shape = (rows, heads, dim)
+    q, qs = _rows3(name, q, dev, shape)
     if max_query_len < 0 or window < 0:
         raise CudaKernelError(ERR_SHAPE, f"{name}: max_query_len {max_query_len}, window {window}")
-    with _on_device(dev):
-        out, lse = _attention_out(name, q, out, out_dtype, return_lse)
-        nbytes = _attention_workspace(heads, kv_heads, dim)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    out, lse = _attention_out(name, dev, shape, q, out, out_dtype, return_lse)
+    nbytes, stream = _attention_workspace(heads, kv_heads, dim), _raw_stream(dev)
+    with _workspace(nbytes, stream) as ws:
         code = _lib.lib().hpc_paged_attention(
-            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), _DTYPE_IDS.get(dt, -1), pages, page_size,
-            page_table.data_ptr(), page_table.shape[1], query_starts.data_ptr(), kv_lens.data_ptr(), seqs, rows, heads,
-            kv_heads, dim, max_query_len, scale, window, ws.data_ptr(), nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype],
-            lse.data_ptr() if return_lse else None, _raw_stream(dev))
+            q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), _DTYPE_IDS.get(dt, -1), pages, page_size,
+            page_table.data_ptr(), width, query_starts.data_ptr(), kv_lens.data_ptr(), seqs, rows, heads, kv_heads, dim,
+            max_query_len, scale, window, ws, nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype],
+            lse.data_ptr() if return_lse else None, stream)
     if code:
         assert_cuda_ok(code, name)
     return (out, lse) if return_lse else out
@@ -525,30 +539,35 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_st
     [rows][kv_heads][head_dim] (f16 or bf16; views with a row stride allowed),
     sequence s = rows query_starts[s] .. query_starts[s+1]."""
     name = "promptAttention"
-    dev, dt = q.device, q.dtype
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or not q.is_cuda:
         raise CudaKernelError(ERR_SHAPE, f"{name}: q, k and v are [rows][heads][head_dim] device tensors")
+    dev, dt = q.get_device(), q.dtype
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return prompt_attention(q, k, v, query_starts, max_query_len=max_query_len, scale=scale, window=window,
+                                    out=out, out_dtype=out_dtype, return_lse=return_lse)
     if k.dtype != dt or v.dtype != dt:
         raise CudaKernelError(ERR_TYPE, f"{name}: queries of {dt}, keys of {k.dtype}, values of {v.dtype}")
-    rows, heads, dim = q.shape
-    kv_heads = k.shape[1]
-    if k.shape[0] != rows:
-        raise CudaKernelError(ERR_SHAPE, f"{name}: {rows} query rows, {k.shape[0]} key rows")
+    shape = rows, heads, dim = q.shape
+    kv_rows, kv_heads, _ = k.shape
+    if kv_rows != rows:
+        raise CudaKernelError(ERR_SHAPE, f"{name}: {rows} query rows, {kv_rows} key rows")
     _check_i32(name, dev, query_starts)
     seqs = query_starts.numel() - 1
     if seqs < 0:
         raise CudaKernelError(ERR_SHAPE, f"{name}: query_starts is empty")
-    q, k, v = _rows3(name, q, dev, heads, dim), _rows3(name, k, dev, kv_heads, dim), _rows3(name, v, dev, kv_heads, dim)
+    q, qs = _rows3(name, q, dev, shape)
+    k, ks = _rows3(name, k, dev, (rows, kv_heads, dim))
+    v, vs = _rows3(name, v, dev, (rows, kv_heads, dim))
     if max_query_len < 0 or window < 0:
         raise CudaKernelError(ERR_SHAPE, f"{name}: max_query_len {max_query_len}, window {window}")
-    with _on_device(dev):
-        out, lse = _attention_out(name, q, out, out_dtype, return_lse)
-        nbytes = _attention_workspace(heads, kv_heads, dim)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    out, lse = _attention_out(name, dev, shape, q, out, out_dtype, return_lse)
+    nbytes, stream = _attention_workspace(heads, kv_heads, dim), _raw_stream(dev)
+    with _workspace(nbytes, stream) as ws:
         code = _lib.lib().hpc_prompt_attention(
-            q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _DTYPE_IDS.get(dt, -1),
-            query_starts.data_ptr(), seqs, rows, heads, kv_heads, dim, max_query_len, scale, window, ws.data_ptr(),
-            nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype], lse.data_ptr() if return_lse else None, _raw_stream(dev))
+            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _DTYPE_IDS.get(dt, -1), query_starts.data_ptr(), seqs,
+            rows, heads, kv_heads, dim, max_query_len, scale, window, ws, nbytes, out.data_ptr(), _DTYPE_IDS[out.dtype],
+            lse.data_ptr() if return_lse else None, stream)
     if code:
         assert_cuda_ok(code, name)
     return (out, lse) if return_lse else out
@@ -579,20 +598,28 @@ def logits_topk(logits: torch.Tensor, k: int, *, history: torch.Tensor | None = 
     [rows][>= ceil(vocab / 32)].  Logits and their history entries stay as
     they are."""
     name = "logitsTopK"
-    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda:
         raise CudaKernelError(ERR_TYPE, f"{name}: logits are [rows][vocab] float32 on a device")
+    dev = logits.get_device()
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return logits_topk(logits, k, history=history, history_starts=history_starts, prompt_lens=prompt_lens,
+                               repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
+                               bias_values=bias_values, bias_starts=bias_starts, allowed=allowed)
     rows, vocab = logits.shape
-    dev = logits.device
-    if logits.stride(1) != 1 or logits.stride(0) < vocab:
+    stride, one = logits.stride()
+    if one != 1 or stride < vocab:
         logits = logits.contiguous()
-    stride = logits.stride(0) if rows > 1 else max(vocab, 1)
+        stride = vocab
+    if rows <= 1:
+        stride = max(vocab, 1)
 
     def ptr(t, dtype, count, what):
         if t is None:
             return None
-        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (count is not None and t.numel() != count):
-            raise CudaKernelError(ERR_SHAPE, f"{name}: {what} is contiguous {dtype} on {dev}"
-                                             + ("" if count is None else f" with {count} values"))
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or (count >= 0 and t.numel() != count):
+            raise CudaKernelError(ERR_SHAPE, f"{name}: {what} is contiguous {dtype} on cuda:{dev}"
+                                             + ("" if count < 0 else f" with {count} values"))
         return t.data_ptr() or None
 
     if (history is None) != (history_starts is None):
@@ -607,18 +634,17 @@ def logits_topk(logits: torch.Tensor, k: int, *, history: torch.Tensor | None = 
         astride = allowed.shape[1]
     hist_n = history.numel() if history is not None else 0
     bias_n = bias_ids.numel() if bias_ids is not None else 0
-    args = (ptr(history, i32, None, "history"), hist_n, ptr(history_starts, i32, rows + 1, "history_starts"),
+    args = (ptr(history, i32, -1, "history"), hist_n, ptr(history_starts, i32, rows + 1, "history_starts"),
             ptr(prompt_lens, i32, rows, "prompt_lens"), ptr(repetition, f32, rows, "repetition"),
             ptr(frequency, f32, rows, "frequency"), ptr(presence, f32, rows, "presence"),
-            ptr(bias_ids, i32, None, "bias_ids"), ptr(bias_values, f32, bias_n, "bias_values"), bias_n,
-            ptr(bias_starts, i32, rows + 1, "bias_starts"), ptr(allowed, i32, None, "allowed"), astride)
-    nbytes = _logits_workspace(rows, vocab, k)
-    with _on_device(dev):
-        ids = torch.empty((rows, k), dtype=i32, device=dev)
-        vals = torch.empty((rows, k), dtype=f32, device=dev)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        code = _lib.lib().hpc_logits_topk(logits.data_ptr(), stride, rows, vocab, k, *args, ws.data_ptr(), nbytes,
-                                          ids.data_ptr(), vals.data_ptr(), _raw_stream(dev))
+            ptr(bias_ids, i32, -1, "bias_ids"), ptr(bias_values, f32, bias_n, "bias_values"), bias_n,
+            ptr(bias_starts, i32, rows + 1, "bias_starts"), ptr(allowed, i32, -1, "allowed"), astride)
+    nbytes, stream = _logits_workspace(rows, vocab, k), _raw_stream(dev)
+    vals = logits.new_empty((rows, k))
+    ids = torch.empty_like(vals, dtype=i32)
+    with _workspace(nbytes, stream) as ws:
+        code = _lib.lib().hpc_logits_topk(logits.data_ptr(), stride, rows, vocab, k, *args, ws, nbytes, ids.data_ptr(),
+                                          vals.data_ptr(), stream)
     if code:
         assert_cuda_ok(code, name)
     return ids, vals
