@@ -6,9 +6,9 @@
 // any number.  The query heads that share a KV head and the new tokens of the
 // sequence are the rows of one product, so each key and value is read once
 // for all of them: per element 2 rows multiply-adds for 2 bytes, which the
-// memory bounds by far up to 16 rows.
+// memory bounds by far up to 24 rows.
 //
-// Work: an item is (sequence, KV head, block of 8 or 16 rows); its keys are cut
+// Work: an item is (sequence, KV head, block of 8, 16 or 24 rows); its keys are cut
 // into tiles of 64, and the tiles of all items, in order, are dealt out
 // evenly to a grid that fills the machine -- a CTA takes a run of tiles, so
 // ragged batches balance to a tile and one long sequence spreads over every
@@ -19,13 +19,14 @@
 //
 // CTA: a producer warp keeps a ring of K and V tiles full by TMA (page by
 // page, each piece of 64 elements 128-byte swizzled), so 100 KB and more are
-// in flight per SM whatever the warps compute.  Four consumer warps take 16
-// keys each of every tile and share nothing until the item ends: S^T = K Q^T
+// in flight per SM whatever the warps compute.  For every 8 rows (16 with heads
+// of 64) four consumer warps take 16 keys each of every tile and share nothing
+// until the item ends: S^T = K Q^T
 // (m16n8k16: the 16 keys are the M side, so 8 rows cost 8 columns instead of
 // a padded 16), the row maxima and sums in f32 over the warp's own keys, P
-// rounded to the cache's type for the second product -- its relative 2^-9
-// (2^-12 for f16) is that of the values it multiplies -- and O^T += V^T P^T in
-// f32 registers.  The warps' four partials are added in shared memory at the end.
+// rounded to the cache's type for the second product -- its relative 2^-8
+// (2^-11 for f16) is that of the values it multiplies -- and O^T += V^T P^T in
+// f32 registers.  The four partials of a row are added in shared memory at the end.
 //
 // A key that a row does not see adds nothing to it, whatever its value
 // holds: values at or behind the sequence's end are zeroed in shared memory
@@ -41,18 +42,27 @@ namespace hc {
 namespace {
 
 constexpr int AR_TILE = 64;      // keys per tile
-constexpr int AR_WARPS = 4;      // consumer warps, 16 keys of a tile each
-constexpr int AR_THREADS = 32 * (AR_WARPS + 1);
+constexpr int AR_WARPS = 4;      // consumer warps of a row group, 16 keys of a tile each
 constexpr float LN2 = 0.6931471805599453f;
 
-template <int D, int NB>
+// Rows of a block: RG groups of 8 NB, each with four consumer warps; the
+// groups share the ring's tiles.
+template <int D, int NB, int RG>
 struct RowsCfg {
-  static constexpr int kSlot = AR_TILE * D * 2;                          // one K or V tile
-  static constexpr int kMergeRow = D + 4;                                // floats; + 4: no bank conflicts
-  static constexpr int kMerge = AR_WARPS * 8 * NB * kMergeRow * 4;
-  // as many tiles in flight as fit beside the merge buffer with 1 / 2 / 3 CTAs per SM
-  static constexpr int kSlots = D == 256 ? (NB == 1 ? 6 : 5) : D == 128 ? (NB == 1 ? 5 : 4) : (NB == 1 ? 8 : 6);
-  static constexpr int kSmem = 1024 + kSlots * kSlot + kMerge;           // + alignment
+  static constexpr int kRows = 8 * NB * RG;
+  static constexpr int kThreads = 32 * (AR_WARPS * RG + 1);
+  static constexpr int kCtas = D == 256 || RG > 2 ? 1 : D == 128 || RG == 2 ? 2 : 3;  // per SM
+  static constexpr int kSlot = AR_TILE * D * 2;                                      // one K or V tile
+  static constexpr int kMergeRow = D + 4;                                            // floats; + 4: no bank conflicts
+  static constexpr int kMergeWarps = RG == 1 ? AR_WARPS : 2;                         // whose rows of a group fit there
+  static constexpr int kMerge = kMergeWarps * kRows * kMergeRow * 4;
+  // fragments of Q^T in shared memory, where registers for them would spill
+  static constexpr bool kQShared = RG > 1;
+  static constexpr int kQ = kQShared ? kRows * D * 2 : 0;
+  // as many tiles in flight as fit beside the merge buffer
+  static constexpr int kFit = (227 * 1024 / kCtas - 2048 - 1024 - kMerge - kQ) / kSlot;
+  static constexpr int kSlots = kFit < 16 ? kFit : 16;
+  static constexpr int kSmem = 1024 + kSlots * kSlot + kMerge + kQ;                       // + alignment
 };
 
 // What the join kernel needs of an item cut by a CTA boundary.
@@ -63,8 +73,8 @@ struct JoinRec {
 };
 
 struct RowsWork {
-  float* o;      // [2 * grid][8 NB][D]
-  float2* ml;    // [2 * grid][8 NB]: maximum (in log2 units), sum
+  float* o;      // [2 * grid][rows of a block][D]
+  float2* ml;    // [2 * grid][rows of a block]: maximum (in log2 units), sum
   JoinRec* rec;  // [grid]
 };
 
@@ -115,13 +125,13 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32
 struct SeqTiles {
   int first, count, blocks;
 };
-template <int NB>
+template <int R>
 __device__ __forceinline__ SeqTiles seq_tiles(const SeqSpan& q, int group, int window) {
   SeqTiles t;
   const int low = window > 0 ? max(0, q.len - q.n - window + 1) : 0;
   t.first = low / AR_TILE;
   t.count = max(1, (q.len + AR_TILE - 1) / AR_TILE - t.first);
-  t.blocks = (q.n * group + 8 * NB - 1) / (8 * NB);
+  t.blocks = (q.n * group + R - 1) / R;
   return t;
 }
 
@@ -131,11 +141,11 @@ __device__ __forceinline__ long long cta_begin(long long total, int c, int grid)
 struct BlockSpan {
   int rows, lo, hi, pos0;
 };
-template <int NB>
+template <int R>
 __device__ __forceinline__ BlockSpan block_span(const SeqSpan& q, int block, int group, int window) {
   BlockSpan s;
-  const int r0 = block * 8 * NB;
-  s.rows = min(8 * NB, q.n * group - r0);
+  const int r0 = block * R;
+  s.rows = min(R, q.n * group - r0);
   s.pos0 = q.len - q.n;  // position of the sequence's first new token
   const int p_first = s.pos0 + r0 / group, p_last = s.pos0 + (r0 + s.rows - 1) / group;
   s.lo = window > 0 ? max(0, p_first - window + 1) : 0;
@@ -160,17 +170,17 @@ __device__ __forceinline__ bool not_finite2<__nv_bfloat16>(uint32_t v) {
   return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
 }
 
-template <class T, int D, int NB>
-__global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
+template <class T, int D, int NB, int RG>
+__global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, RG>::kCtas)
     hc_attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const __grid_constant__ RowsArgs p) {
-  using Cfg = RowsCfg<D, NB>;
-  constexpr int R = 8 * NB, KS = D / 16;
+  using Cfg = RowsCfg<D, NB, RG>;
+  constexpr int R = Cfg::kRows, GR = 8 * NB, KS = D / 16, WARPS = AR_WARPS * RG;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[Cfg::kSlots], empty[Cfg::kSlots];
-  __shared__ long long s_sum[AR_WARPS + 1];
+  __shared__ long long s_sum[Cfg::kThreads / 32];
   __shared__ Walk s_walk;
-  __shared__ float2 s_ml[AR_WARPS][R];
+  __shared__ float2 s_ml[WARPS][GR];
   const int t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
   const int grid = int(gridDim.x), cta = int(blockIdx.x);
   const int group = p.a.heads / p.a.kv_heads, window = p.a.window;
@@ -179,14 +189,14 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
   if (t == 0) {
     for (int i = 0; i < Cfg::kSlots; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], AR_WARPS);
+      mbar_init(&empty[i], WARPS);
     }
   }
   pdl_launch_next();
   pdl_wait_prior();
 
   // ---- this CTA's run of tiles: thread t counts sequences [t * per, ...)
-  const int per = (p.b.seqs + AR_THREADS - 1) / AR_THREADS;
+  const int per = (p.b.seqs + Cfg::kThreads - 1) / Cfg::kThreads;
   long long mine = 0;
   bool any_bad = false;
   for (int i = 0; i < per; ++i) {
@@ -195,7 +205,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
     bool bad;
     const SeqSpan q = seq_span(p.b, s, &bad);
     any_bad = any_bad || bad;
-    const SeqTiles st = seq_tiles<NB>(q, group, window);
+    const SeqTiles st = seq_tiles<R>(q, group, window);
     mine += (long long)p.a.kv_heads * st.blocks * st.count;
   }
   if (any_bad && p.a.err) atomicExch(p.a.err, DEVICE_ERR_PAGE);
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
   __syncthreads();
   long long total = 0;
 #pragma unroll
-  for (int i = 0; i <= AR_WARPS; ++i) {
+  for (int i = 0; i < Cfg::kThreads / 32; ++i) {
     if (i < warp) incl += s_sum[i];
     total += s_sum[i];
   }
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
     long long at = incl - mine;
     for (int s = t * per;; ++s) {
       bool bad;
-      const SeqTiles st = seq_tiles<NB>(seq_span(p.b, s, &bad), group, window);
+      const SeqTiles st = seq_tiles<R>(seq_span(p.b, s, &bad), group, window);
       const long long n = (long long)p.a.kv_heads * st.blocks * st.count;
       if (u0 < at + n) {
         const long long d = u0 - at;
@@ -242,17 +252,17 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
 
   int it = 0;  // K and V tiles so far: slot it % kSlots, phase it / kSlots
   bool ok = true;
-  if (warp == AR_WARPS) {
+  if (warp == WARPS) {
     // ---- producer: lane i looks up the tile's i-th page; one lane issues the
     // copies, with operands that are uniform in the warp (elect_one)
     const int box = p.box_rows, box_shift = __ffs(box) - 1, ppt = AR_TILE >> box_shift;
     while (w.u < w.end && ok) {
       bool bad;
       const SeqSpan q = seq_span(p.b, w.s, &bad);
-      const SeqTiles st = seq_tiles<NB>(q, group, window);
+      const SeqTiles st = seq_tiles<R>(q, group, window);
       for (; w.head < p.a.kv_heads && w.u < w.end && ok; ++w.head, w.block = 0) {
         for (; w.block < st.blocks && w.u < w.end && ok; ++w.block, w.tile = 0) {
-          const BlockSpan sp = block_span<NB>(q, w.block, group, window);
+          const BlockSpan sp = block_span<R>(q, w.block, group, window);
           for (; w.tile < st.count && w.u < w.end && ok; ++w.tile, ++w.u) {
             const int k0 = (st.first + w.tile) * AR_TILE;
             if (k0 + AR_TILE <= sp.lo || k0 >= sp.hi) continue;
@@ -302,36 +312,48 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
 
   // ---- consumers
   const int lr = lane >> 2, lc = lane & 3;
+  const int rg = warp / AR_WARPS, kw = warp % AR_WARPS;  // row group, and the keys' quarter
   const int box_shift = __ffs(p.box_rows) - 1;
   // byte offset of key row j of a tile (its first 128-byte piece); pieces are box_rows * 128 apart
   const auto row_off = [&](int j) { return (j >> box_shift) * (p.box_rows * D * 2) + (j & (p.box_rows - 1)) * 128; };
   const int piece = p.box_rows * 128;
+  const auto group_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + rg), "n"(32 * AR_WARPS) : "memory"); };
   // this lane's ldmatrix rows (fixed within the tile) and 16-byte chunks
-  const int kj = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
-  const int vj = warp * 16 + (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
+  const int kj = kw * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
+  const int vj = kw * 16 + (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
   const uint32_t koff = uint32_t(row_off(kj)), voff = uint32_t(row_off(vj));
   while (w.u < w.end) {
     bool bad;
     const SeqSpan q = seq_span(p.b, w.s, &bad);
-    const SeqTiles st = seq_tiles<NB>(q, group, window);
+    const SeqTiles st = seq_tiles<R>(q, group, window);
     for (; w.head < p.a.kv_heads && w.u < w.end; ++w.head, w.block = 0) {
       for (; w.block < st.blocks && w.u < w.end; ++w.block, w.tile = 0) {
-        const BlockSpan sp = block_span<NB>(q, w.block, group, window);
-        const int r0 = w.block * R;
+        const BlockSpan sp = block_span<R>(q, w.block, group, window);
+        const int r0 = w.block * R + rg * GR;               // this group's first row
+        const int rows = min(GR, sp.rows - rg * GR);        // none: below 1
         // B fragments of Q^T, straight from the rows
-        uint32_t qf[NB][KS][2];
+        uint32_t qf[Cfg::kQShared ? 1 : NB][KS][2];
+        uint2* qs = reinterpret_cast<uint2*>(merge + Cfg::kMerge / 4) + rg * NB * KS * 32;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int r = r0 + nb * 8 + lr;
-          const bool in = r - r0 < sp.rows;
+          const bool in = r - r0 < rows;
           const T* src = static_cast<const T*>(p.a.q) + int64_t(q.row0 + (in ? r / group : 0)) * p.a.q_stride +
                          (w.head * group + (in ? r % group : 0)) * D + lc * 2;
+          if constexpr (Cfg::kQShared) {
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            qf[nb][k][0] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
-            qf[nb][k][1] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
+            for (int k = kw; k < KS; k += AR_WARPS)
+              qs[(k * NB + nb) * 32 + lane] = make_uint2(in ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u,
+                                                         in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u);
+          } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              qf[nb][k][0] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+              qf[nb][k][1] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
+            }
           }
         }
+        if constexpr (Cfg::kQShared) group_sync();
         // keys [low, lim] of this lane's two rows of every 8
         int lim[NB][2], low[NB][2];
         float m[NB][2], l[NB][2];
@@ -342,7 +364,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
           for (int e = 0; e < 2; ++e) {
             const int r = nb * 8 + lc * 2 + e;
             const int pos = sp.pos0 + (r0 + r) / group;
-            lim[nb][e] = r < sp.rows ? min(pos, q.len - 1) : -1;
+            lim[nb][e] = r < rows ? min(pos, q.len - 1) : -1;
             low[nb][e] = window > 0 ? pos - window + 1 : 0;
             m[nb][e] = -INFINITY;
             l[nb][e] = 0.0f;
@@ -353,16 +375,16 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
           for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nb][k][e] = 0.0f;
-        // every key of [all_lo, all_hi] is seen by every row of the block
+        // every key of [all_lo, all_hi] is seen by every row of the group
         const int all_hi = min(q.len - 1, sp.pos0 + r0 / group);
-        const int all_lo = window > 0 ? sp.pos0 + (r0 + sp.rows - 1) / group - window + 1 : 0;
+        const int all_lo = window > 0 ? sp.pos0 + (r0 + rows - 1) / group - window + 1 : 0;
         const int tile0 = w.tile;
         for (; w.tile < st.count && w.u < w.end; ++w.tile, ++w.u) {
           const int k0 = (st.first + w.tile) * AR_TILE;
           // after a wait gave up the warp only walks on, to meet the others at the barriers
           if (!ok || k0 + AR_TILE <= sp.lo || k0 >= sp.hi) continue;
-          const int j0 = k0 + warp * 16;  // this warp's keys
-          const bool idle = j0 >= sp.hi || j0 + 16 <= sp.lo;
+          const int j0 = k0 + kw * 16;  // this warp's keys
+          const bool idle = rows < 1 || j0 >= sp.hi || j0 + 16 <= sp.lo;
           const int ks = it % Cfg::kSlots, kph = it / Cfg::kSlots;
           const int vs = (it + 1) % Cfg::kSlots, vph = (it + 1) / Cfg::kSlots;
           it += 2;
@@ -385,7 +407,14 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
               uint32_t af[4];
               ldsm4(af, kb + (k >> 2) * piece + ((((k & 3) * 2 + kc) ^ (kj & 7)) << 4));
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma16<T>(s[k & 1][nb], af, qf[nb][k][0], qf[nb][k][1]);
+              for (int nb = 0; nb < NB; ++nb) {
+                if constexpr (Cfg::kQShared) {
+                  const uint2 f = qs[(k * NB + nb) * 32 + lane];
+                  mma16<T>(s[k & 1][nb], af, f.x, f.y);
+                } else {
+                  mma16<T>(s[k & 1][nb], af, qf[nb][k][0], qf[nb][k][1]);
+                }
+              }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[ks]);
@@ -438,7 +467,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
             if (j0 + 15 > all_hi || j0 < all_lo) {  // some row does not see some of these keys
               bool odd = false;
               for (int i = lane; i < 16 * (D / 8); i += 32) {
-                const int jj = i / (D / 8), c = i % (D / 8), j = warp * 16 + jj;
+                const int jj = i / (D / 8), c = i % (D / 8), j = kw * 16 + jj;
                 const uint32_t at = vt + row_off(j) + (c >> 3) * piece + (((c & 7) ^ (j & 7)) << 4);
                 if (j0 + jj >= q.len) {
                   asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
@@ -469,7 +498,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
               for (int jj = 0; jj < 16; ++jj) {
                 const int j = j0 + jj;
                 if (j >= q.len) break;
-                const int rj = warp * 16 + jj;
+                const int rj = kw * 16 + jj;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -509,39 +538,83 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
             v += __shfl_xor_sync(0xffffffffu, v, 16);
             if (lr == 0) s_ml[warp][nb * 8 + lc * 2 + e] = make_float2(m[nb][e], v);
           }
-        float* mb = merge + warp * R * Cfg::kMergeRow;
+        // one group: its four warps lay their sums out as rows and write the
+        // rows' total.  More groups have room for two warps' rows each: two
+        // warps hand their sums to the other two first, in the fragments' own
+        // layout (for one group that costs 2.5 us of a token's 11.6).
+        constexpr int MW = Cfg::kMergeWarps;
+        float* mb = merge + rg * MW * GR * Cfg::kMergeRow;
+        if (MW == 2 && kw >= 2) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mb[(nb * 8 + lc * 2 + (e & 1)) * Cfg::kMergeRow + k * 16 + (e >> 1) * 8 + lr] = o[nb][k][e];
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * AR_WARPS) : "memory");
+            for (int k = 0; k < KS; ++k)
+              *reinterpret_cast<float4*>(mb + (((kw - 2) * NB + nb) * KS + k) * 128 + lane * 4) =
+                  make_float4(o[nb][k][0], o[nb][k][1], o[nb][k][2], o[nb][k][3]);
+        }
+        if constexpr (MW == 2) group_sync();
         const bool whole = tile0 == 0 && w.tile == st.count;
         const int part = tile0 > 0 ? 2 * cta : 2 * cta + 1;
-        constexpr int TPR = 32 * AR_WARPS / R;  // threads per row
-        {
-          const int r = t / TPR, c = t % TPR;
-          float mx = -INFINITY;
+        // a row's maximum, the warps' factors against it, and its sum
+        const auto row_stats = [&](int r, float (&f)[AR_WARPS], float& mx) {
+          mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < AR_WARPS; ++i) mx = fmaxf(mx, s_ml[i][r].x);
+          for (int i = 0; i < AR_WARPS; ++i) mx = fmaxf(mx, s_ml[rg * AR_WARPS + i][r].x);
           const float ms = mx == -INFINITY ? 0.0f : mx;
-          float f[AR_WARPS], sum = 0.0f;
+          float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < AR_WARPS; ++i) {
-            f[i] = ex2(s_ml[i][r].x - ms);
-            sum += f[i] * s_ml[i][r].y;
+            const float2 v = s_ml[rg * AR_WARPS + i][r];
+            f[i] = ex2(v.x - ms);
+            sum += f[i] * v.y;
           }
-          if (r < sp.rows) {
+          return sum;
+        };
+        if (MW == 2 && kw < 2) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float fa[2], fb[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float f[AR_WARPS], mx;
+              row_stats(nb * 8 + lc * 2 + e, f, mx);
+              fa[e] = kw ? f[1] : f[0], fb[e] = kw ? f[3] : f[2];
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              const float4 x = *reinterpret_cast<const float4*>(mb + ((kw * NB + nb) * KS + k) * 128 + lane * 4);
+              o[nb][k][0] = fa[0] * o[nb][k][0] + fb[0] * x.x, o[nb][k][1] = fa[1] * o[nb][k][1] + fb[1] * x.y;
+              o[nb][k][2] = fa[0] * o[nb][k][2] + fb[0] * x.z, o[nb][k][3] = fa[1] * o[nb][k][3] + fb[1] * x.w;
+            }
+          }
+        }
+        if constexpr (MW == 2) group_sync();
+        if (kw < MW) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                mb[(kw * GR + nb * 8 + lc * 2 + (e & 1)) * Cfg::kMergeRow + k * 16 + (e >> 1) * 8 + lr] = o[nb][k][e];
+        }
+        group_sync();
+        constexpr int TPR = 32 * AR_WARPS / GR;  // threads per row
+        {
+          const int tg = kw * 32 + lane, r = tg / TPR, c = tg % TPR;
+          if (r < rows) {
+            float f[AR_WARPS], mx;
+            const float sum = row_stats(r, f, mx);
             const int row = q.row0 + (r0 + r) / group, head = w.head * group + (r0 + r) % group;
+            const int64_t prow = int64_t(part) * R + rg * GR + r;
             const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
             for (int d = c * 4; d < D; d += TPR * 4) {
               float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-              for (int i = 0; i < AR_WARPS; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(merge + (i * R + r) * Cfg::kMergeRow + d);
-                v.x += f[i] * x.x, v.y += f[i] * x.y, v.z += f[i] * x.z, v.w += f[i] * x.w;
+              for (int i = 0; i < MW; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(mb + (i * GR + r) * Cfg::kMergeRow + d);
+                const float g = MW == 2 ? 1.0f : f[i];
+                v.x += g * x.x, v.y += g * x.y, v.z += g * x.z, v.w += g * x.w;
               }
               if (whole) {
                 const int64_t at = (int64_t(row) * p.a.heads + head) * D + d;
@@ -552,11 +625,11 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
                   *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + at) =
                       make_uint2(HalfOps<T>::pack(v.x * inv, v.y * inv), HalfOps<T>::pack(v.z * inv, v.w * inv));
               } else {
-                *reinterpret_cast<float4*>(p.w.o + (int64_t(part) * R + r) * D + d) = v;
+                *reinterpret_cast<float4*>(p.w.o + prow * D + d) = v;
               }
             }
             if (c == 0) {
-              if (!whole) p.w.ml[part * R + r] = make_float2(mx, sum);
+              if (!whole) p.w.ml[prow] = make_float2(mx, sum);
               else if (p.a.lse) p.a.lse[int64_t(row) * p.a.heads + head] = sum == 0.0f ? -INFINITY : LN2 * (mx + log2f(sum));
             }
           }
@@ -570,7 +643,7 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
           r.total = total;
           p.w.rec[cta] = r;
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * AR_WARPS) : "memory");
+        group_sync();
       }
       if (w.block < st.blocks) break;
     }
@@ -584,16 +657,16 @@ __global__ void __launch_bounds__(AR_THREADS, D == 256 ? 1 : D == 128 ? 2 : 3)
 // that take every GROUPS-th partial each (one long sequence leaves a partial on
 // every SM), added up in the groups' order.
 constexpr int AJ_THREADS = 256, AJ_PARTS = 512;
-template <class T, int D, int NB>
+template <class T, int D, int R>
 __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_constant__ RowsArgs p, int grid) {
-  constexpr int R = 8 * NB, LANES = D / 4, GROUPS = AJ_THREADS / LANES;
+  constexpr int LANES = D / 4, GROUPS = AJ_THREADS / LANES;
   __shared__ int s_part[AJ_PARTS];
   __shared__ float2 s_ml[AJ_PARTS];
   __shared__ int s_n;
   __shared__ float s_max[AJ_THREADS / 32];
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ float s_sum[GROUPS];
-  const int c0 = int(blockIdx.x), r = int(blockIdx.y), t = int(threadIdx.x);
+  const int c0 = int(blockIdx.x), t = int(threadIdx.x);
   pdl_wait_prior();
   const JoinRec rec = p.w.rec[c0];
   if (rec.block < 0) return;
@@ -601,6 +674,7 @@ __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_c
   const SeqSpan q = seq_span(p.b, rec.seq, &bad);
   const int group = p.a.heads / p.a.kv_heads;
   const int r0 = rec.block * R;
+  const int r = int(blockIdx.y);
   if (r >= min(R, q.n * group - r0)) return;
   // the partials, in CTA order; a CTA that held no tile left none
   if (t < 32) {
@@ -664,29 +738,32 @@ __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_c
 
 // CTAs per SM times the SMs, of which the workspace allows for 160.
 constexpr int kMaxSms = 160;
-constexpr int ctas_per_sm(int dim) { return dim == 256 ? 1 : dim == 128 ? 2 : 3; }
-
 size_t ws_bytes(int grid, int rows, int dim) {
   const auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   return al(size_t(2 * grid) * rows * dim * 4) + al(size_t(2 * grid) * rows * 8) + al(size_t(grid) * sizeof(JoinRec));
 }
 
-template <class T, int D, int NB>
+template <int D, int NB, int RG>
+size_t rows_ws() {
+  return ws_bytes(kMaxSms * RowsCfg<D, NB, RG>::kCtas, RowsCfg<D, NB, RG>::kRows, D);
+}
+
+template <class T, int D, int NB, int RG>
 cudaError_t launch_rows(RowsArgs& p, const KvSource& kv, void* workspace, cudaStream_t st) {
-  using Cfg = RowsCfg<D, NB>;
-  auto kernel = hc_attn_rows_kernel<T, D, NB>;
+  using Cfg = RowsCfg<D, NB, RG>;
+  auto kernel = hc_attn_rows_kernel<T, D, NB, RG>;
   static std::atomic<uint64_t> attr{0};
   cudaError_t e = once_per_current_device(attr, [&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   });
   if (e != cudaSuccess) return e;
-  const int grid = std::min(kMaxSms, sm_count()) * ctas_per_sm(D);
+  const int grid = std::min(kMaxSms, sm_count()) * Cfg::kCtas;
   const auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.w.o = reinterpret_cast<float*>(ws);
-  ws += al(size_t(2 * grid) * 8 * NB * D * 4);
+  ws += al(size_t(2 * grid) * Cfg::kRows * D * 4);
   p.w.ml = reinterpret_cast<float2*>(ws);
-  ws += al(size_t(2 * grid) * 8 * NB * 8);
+  ws += al(size_t(2 * grid) * Cfg::kRows * 8);
   p.w.rec = reinterpret_cast<JoinRec*>(ws);
   p.box_rows = p.b.table ? std::min(AR_TILE, 1 << p.b.page_shift) : AR_TILE;
   p.slots = int64_t(kv.slots);
@@ -695,18 +772,27 @@ cudaError_t launch_rows(RowsArgs& p, const KvSource& kv, void* workspace, cudaSt
   if (e == cudaSuccess)
     e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, p.box_rows, D / 64);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(grid), dim3(AR_THREADS), Cfg::kSmem, st, km, vm, p);
+  e = launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, st, km, vm, p);
   if (e != cudaSuccess) return e;
   static_assert(3 * kMaxSms <= AJ_PARTS, "one partial per CTA at most");
-  return launch_pdl(hc_attn_join_kernel<T, D, NB>, dim3(grid, 8 * NB), dim3(AJ_THREADS), 0, st, p, grid);
+  return launch_pdl(hc_attn_join_kernel<T, D, Cfg::kRows>, dim3(grid, Cfg::kRows), dim3(AJ_THREADS), 0, st, p, grid);
 }
 
 template <class T, int D>
 cudaError_t launch_rows_d(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_t st) {
-  // 8 rows hold a group of up to 8 heads at one token each; more new tokens
-  // or a larger group fill 16, which halves the times the keys are read
-  return int64_t(p.a.max_q) * (p.a.heads / p.a.kv_heads) <= 8 ? launch_rows<T, D, 1>(p, kv, ws, st)
-                                                              : launch_rows<T, D, 2>(p, kv, ws, st);
+  // Up to 24 rows one block holds all of a KV head's queries and the keys are
+  // read once: 20 rows of 16 sequences of 1000 to 4096 keys take 34 us at
+  // head_dim 256, 87 at 32 / 8 heads of 128 and 2000 to 8000 keys; in two
+  // blocks of 16 they took 45 and 110.  Heads of 64 read so little that more
+  // CTAs with 16 rows in one group win there (20 rows: 74 us against 80).
+  const int64_t rows = int64_t(p.a.max_q) * (p.a.heads / p.a.kv_heads);
+  if (rows <= 8) return launch_rows<T, D, 1, 1>(p, kv, ws, st);
+  if constexpr (D == 64) {
+    return launch_rows<T, D, 2, 1>(p, kv, ws, st);
+  } else {
+    if (rows <= 16 || (rows > 24 && rows <= 32)) return launch_rows<T, D, 1, 2>(p, kv, ws, st);
+    return launch_rows<T, D, 1, 3>(p, kv, ws, st);
+  }
 }
 
 template <class T>
@@ -722,7 +808,9 @@ cudaError_t launch_rows_t(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_
 
 size_t attn_rows_workspace_bytes(int heads, int kv_heads, int dim) {
   (void)heads, (void)kv_heads;
-  return ws_bytes(kMaxSms * ctas_per_sm(dim), 16, dim);
+  return dim == 64 ? std::max(rows_ws<64, 1, 1>(), rows_ws<64, 2, 1>())
+         : dim == 128 ? std::max({rows_ws<128, 1, 1>(), rows_ws<128, 1, 2>(), rows_ws<128, 1, 3>()})
+                      : std::max({rows_ws<256, 1, 1>(), rows_ws<256, 1, 2>(), rows_ws<256, 1, 3>()});
 }
 
 cudaError_t launch_attn_rows(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
