@@ -123,6 +123,10 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 cudaError_t encode_kv_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t slots,
                           uint64_t stride, int heads, int dim, int box_rows, int box_pieces);
 
+// The same for dimensions, strides (bytes) and box of one's own.
+cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box);
+
 template <class... KArgs, class... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                               Args&&... args) {
@@ -162,12 +166,14 @@ struct KvSource {
   int dtype;
 };
 
-size_t attn_rows_workspace_bytes(int heads, int kv_heads, int dim);
+size_t attn_rows_workspace_bytes(int dim);
 cudaError_t launch_attn_rows(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
                              cudaStream_t st);
 
 // Many query rows per sequence, on the tensor cores (hc_prompt_attn.cu).
-cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, cudaStream_t st);
+size_t attn_prompt_workspace_bytes(int dim);
+cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
+                               cudaStream_t st);
 
 }  // namespace hc
 

@@ -790,7 +790,7 @@ cudaError_t launch_rows_d(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_
   if constexpr (D == 64) {
     return launch_rows<T, D, 2, 1>(p, kv, ws, st);
   } else {
-    if (rows <= 16 || (rows > 24 && rows <= 32)) return launch_rows<T, D, 1, 2>(p, kv, ws, st);
+    if (rows <= 16 || rows > 24) return launch_rows<T, D, 1, 2>(p, kv, ws, st);
     return launch_rows<T, D, 1, 3>(p, kv, ws, st);
   }
 }
@@ -806,8 +806,7 @@ cudaError_t launch_rows_t(RowsArgs& p, const KvSource& kv, void* ws, cudaStream_
 
 }  // namespace
 
-size_t attn_rows_workspace_bytes(int heads, int kv_heads, int dim) {
-  (void)heads, (void)kv_heads;
+size_t attn_rows_workspace_bytes(int dim) {
   return dim == 64 ? std::max(rows_ws<64, 1, 1>(), rows_ws<64, 2, 1>())
          : dim == 128 ? std::max({rows_ws<128, 1, 1>(), rows_ws<128, 1, 2>(), rows_ws<128, 1, 3>()})
                       : std::max({rows_ws<256, 1, 1>(), rows_ws<256, 1, 2>(), rows_ws<256, 1, 3>()});
@@ -824,8 +823,8 @@ cudaError_t launch_attn_rows(const AttnArgs& a, const PagedBatch& b, const KvSou
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (the
 // library does not link the driver library itself).
-cudaError_t encode_kv_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t slots,
-                          uint64_t stride, int heads, int dim, int box_rows, int box_pieces) {
+cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -840,14 +839,19 @@ cudaError_t encode_kv_map(CUtensorMap* map, CUtensorMapDataType type, const void
     encode = reinterpret_cast<Encode>(fn);
     cached.store(encode);
   }
-  const cuuint64_t dims[3] = {64, slots, cuuint64_t(heads) * (dim / 64)};
-  const cuuint64_t strides[2] = {stride * 2, 128};
-  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(box_pieces)};
-  const cuuint32_t ones[3] = {1, 1, 1};
-  const CUresult r = encode(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, ones,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t encode_kv_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t slots,
+                          uint64_t stride, int heads, int dim, int box_rows, int box_pieces) {
+  const cuuint64_t dims[3] = {64, slots, cuuint64_t(heads) * (dim / 64)};
+  const cuuint64_t strides[2] = {stride * 2, 128};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(box_pieces)};
+  return encode_map(map, type, 3, base, dims, strides, box);
 }
 
 }  // namespace hc
@@ -886,6 +890,10 @@ hc::PagedBatch hpc_paged_batch(const int32_t* starts, const int32_t* lens, const
 
 namespace {
 
+size_t workspace_need(size_t head_dim) {
+  return std::max(hc::attn_rows_workspace_bytes(int(head_dim)), hc::attn_prompt_workspace_bytes(int(head_dim)));
+}
+
 int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSource& kv, hc::PagedBatch b,
               size_t heads, size_t kv_heads, size_t head_dim, size_t max_query_len, float scale, size_t window,
               void* d_workspace, size_t workspace_bytes, void* d_out, int out_dtype, float* d_lse, void* stream) {
@@ -905,7 +913,7 @@ int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSo
   const auto off = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
   if (off(d_q) || off(kv.k) || off(kv.v) || off(d_out) || off(d_workspace))
     return hpc_fail(HPC_ERR_ARG, "%s: tensors must be aligned to 16 bytes", what);
-  const size_t need = hc::attn_rows_workspace_bytes(int(heads), int(kv_heads), int(head_dim));
+  const size_t need = workspace_need(head_dim);
   if (workspace_bytes < need)
     return hpc_fail(HPC_ERR_SHAPE, "%s: a workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   hc::AttnArgs a{};
@@ -920,10 +928,13 @@ int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSo
   a.max_q = int(std::min(max_query_len, size_t(b.rows)));
   a.err = hc::device_status_word();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Up to 64 rows (new tokens x heads of a group) the keys are read at most
-  // four times; beyond, a tensor-core tile of 128 rows pays.
-  const bool few = int64_t(a.max_q) * (a.heads / a.kv_heads) <= 64;
-  HPC_CK(few ? hc::launch_attn_rows(a, b, kv, d_workspace, st) : hc::launch_attn_prompt(a, b, kv, st), what);
+  // Rows (new tokens x heads of a group) of a sequence: few go to the kernel
+  // that the keys' bytes bound, more to tensor-core tiles of 128 rows.  16
+  // sequences of 2000 to 8000 keys, 32 / 8 heads of 128: 20 rows 88 us there and 101
+  // here, 32 rows 115 and 101, 64 rows 226 and 102; 1000 to 4096 keys, 8 / 2 heads
+  // of 256: 20 rows 34 and 43, 32 rows 40 and 43, 48 rows 49 and 43.
+  const bool few = int64_t(a.max_q) * (a.heads / a.kv_heads) <= (a.dim == 256 ? 32 : 24);
+  HPC_CK(few ? hc::launch_attn_rows(a, b, kv, d_workspace, st) : hc::launch_attn_prompt(a, b, kv, d_workspace, st), what);
   return HPC_OK;
 }
 
@@ -934,7 +945,7 @@ extern "C" {
 int hpc_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t head_dim, size_t *out_bytes) {
   if (int rc = hpc_paged_check("attention workspace", heads, kv_heads, head_dim, 0, 0, 0, 0, 0)) return rc;
   if (!out_bytes) return hpc_fail(HPC_ERR_ARG, "null pointer");
-  *out_bytes = hc::attn_rows_workspace_bytes(int(heads), int(kv_heads), int(head_dim));
+  *out_bytes = workspace_need(head_dim);
   return HPC_OK;
 }
 

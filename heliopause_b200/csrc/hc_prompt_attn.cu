@@ -32,9 +32,18 @@
 // At head_dim 256 P takes the place of its S.
 //
 // The CTAs stay: each takes its next item (sequence, KV head, rows) from the
-// launch by clusterlaunchcontrol while it works on the present one, the
-// longest sums first, and loads its Q, K and V ahead, so that only the rows'
-// store falls between two items.
+// launch by clusterlaunchcontrol shortly before the present one's last keys, the
+// longest sums first, and loads its Q, K and V ahead.  Four warps store an
+// item's rows while the softmax warps are at the next item's tiles.  Twelve
+// prompts of 1 to 2048 tokens (1576 items of 6 tiles on average) take 233 us so;
+// with the rows stored by the softmax warps, Q brought by threads and the next item
+// taken one ahead it was 266 (8192 tokens at head_dim 256: 220 and 250).
+//
+// Few items over long keys (chunks of one long prompt) are cut along the keys:
+// an item gets as many parts as its share of all tiles fills CTAs, each
+// at least 8 tiles; parts leave their sums in the workspace and
+// hc_prompt_join_kernel adds them up.  512 rows x 8 / 2 heads of 256 over 8192 keys:
+// 93 us whole, 42 in parts.
 //
 // K and V arrive by TMA, page by page or straight from packed rows, 128-byte
 // swizzled, which is the operand layout of both products (K rows are K-major; V is
@@ -53,6 +62,9 @@ namespace {
 
 constexpr int PR_KEYS = 128;     // keys per tile
 constexpr int PR_ROWS = 128;     // rows per CTA
+constexpr int PR_AHEAD = 3;      // tiles that are left to load of an item when the next is asked for
+constexpr int PR_PART = 8;       // tiles in a part of an item's keys, at least
+constexpr int PR_PLACES = 2;     // parts that a launch may have for each CTA (pair) of the machine
 constexpr float PR_GROW = 8.0f;  // log2 units a maximum may grow before O is rescaled
 
 template <int D>
@@ -60,20 +72,22 @@ struct PrCfg {
   static constexpr int CG = D == 64 ? 1 : 2;              // CTAs per MMA
   static constexpr bool kOwnP = D <= 128;                 // P beside S, not over it
   static constexpr uint32_t kTmemO = D == 256 ? 256 : 384;
-  static constexpr int kThreads = 512;                    // 8 softmax warps; K, V, S, O and item warps, 3 more loaders
+  static constexpr int kThreads = 512;                    // 8 softmax warps; one each for K, V, S and O; 4 for items
   static constexpr int kQ = PR_ROWS * D * 2;              // bytes of Q
   static constexpr int kK = PR_KEYS / CG * D * 2;         // bytes of K and of V per stage in this CTA
   static constexpr int kStages = D == 256 ? 2 : 4;
-  static constexpr int kStage = 8 * 32 * 64;              // output staging: 32 rows x 64 bytes per warp
-  static constexpr int kSmem = 1024 + kQ + 2 * kStages * kK + kStage;
+  static constexpr int kRowBytes = D == 256 ? 64 : 128;   // output staging: of each of a warp's 32 rows
+  static constexpr int kStage = 4 * 32 * kRowBytes;
+  static constexpr int kQs = D == 256 ? 1 : 2;            // Q of the present item, and of the next where there is room
+  static constexpr int kSmem = 1024 + kQs * kQ + 2 * kStages * kK + kStage;
   static constexpr int kKeys = PR_KEYS / CG;              // keys of K in this CTA
   static constexpr int kPieces = D / 64;                  // 128-byte pieces of a row
   static constexpr int kPiecesV = kPieces / CG;           // of them V pieces in this CTA
   __host__ __device__ static constexpr uint32_t p_col(uint32_t slot) { return kOwnP ? 256 + slot * 64 : slot * 128; }
 };
-// registers per thread: launched with 128, the two softmax warpgroups take 208
+// registers per thread: launched with 128, the two softmax warpgroups take 184
 // (a row of 128 scores each) from the other two
-constexpr int PR_REGS_SOFTMAX = 208, PR_REGS_OTHER = 48;
+constexpr int PR_REGS_SOFTMAX = 184, PR_REGS_OTHER = 72;
 static_assert(2 * PR_REGS_SOFTMAX + 2 * PR_REGS_OTHER == 4 * 128, "the split is of what the block was launched with");
 
 struct PrArgs {
@@ -85,6 +99,13 @@ struct PrArgs {
   int box_k, box_v;    // key rows per TMA copy, as powers of two
   int whole_k, whole_v;  // a copy brings the CTA's whole tile, every piece of it
   int64_t slots;
+  int items;             // items of the launch at most
+  int split;             // most parts that an item's keys are cut into
+  int workers;           // CTAs (or pairs) that the machine runs at a time
+  int q_copy;            // Q comes by TMA
+  float* part_o;         // [place][32 rows][head_dim / 4][row] float4, not divided by the sum
+  float2* part_ml;       // [place][SPAN rows]: maximum (in log2 units) and sum
+  struct PrJoin* join;   // [item]
 };
 
 // ---- tcgen05 -----------------------------------------------------------------
@@ -197,32 +218,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// 2^x for a pair on the FMA pipe: x = n + f with n the nearest integer (in the
-// low bits after adding 1.5 * 2^23), a polynomial of degree 4 for 2^f on
-// [-1/2, 1/2] (the minimax one for the relative error, 2.6e-6, by Remez
-// exchange), and n added to the exponent.  x is at most 8 here and
-// taken as -126 where it is less.  The special-function unit delivers 16
-// results per clock and SM, one tile's exponentials take as long as a
-// head_dim 128 tile's products; every PR_POLY_EVERY-th pair goes this way.
-constexpr int PR_POLY_EVERY = 1000;
-__device__ __forceinline__ void ex2_poly2(uint64_t x, float& e0, float& e1) {
-  float a, b;
-  unpack2(x, a, b);
-  const uint64_t y = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t t = add2(y, pack2(12582912.0f, 12582912.0f));
-  const uint64_t n = add2(t, pack2(-12582912.0f, -12582912.0f));
-  const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), y);
-  uint64_t q = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
-  q = fma2(q, f, pack2(0.240247443318367f, 0.240247443318367f));
-  q = fma2(q, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1;
-  unpack2(t, t0, t1);
-  unpack2(q, e0, e1);
-  e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(t1) << 23));
 }
 
 // ---- barriers across a CTA pair -------------------------------------------------
@@ -340,6 +335,20 @@ __device__ __forceinline__ void pr_tma(uint32_t dst, const CUtensorMap* map, int
         : "memory");
   }
 }
+template <int CG>
+__device__ __forceinline__ void pr_tma_q(uint32_t dst, const CUtensorMap* map, int piece, int head, int token, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(piece), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(piece), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+}
 constexpr uint32_t kLeaderMask = 0xfeffffffu;  // a shared::cluster address in the pair's even CTA
 
 // ---- the tile's sums by plain loops -----------------------------------------------
@@ -347,8 +356,8 @@ constexpr uint32_t kLeaderMask = 0xfeffffffu;  // a shared::cluster address in t
 // One row of a tile, from global memory: keys [lo, hi] of sequence `s`.  Only
 // for tiles where a value that some rows do not see is not finite.
 template <class T, int D>
-__device__ __noinline__ void pr_plain_row(const PrArgs& p, int s, int row0, int kv_head, const T* q, int lo, int hi,
-                                          T* out, float* out32, float* lse) {
+__device__ __forceinline__ void pr_plain_row(const PrArgs& p, int s, int row0, int kv_head, const T* q, int lo, int hi,
+                                          T* out, float* out32, float* lse, float2* part) {
   const auto at = [&](const void* base, int64_t stride, int j) {
     int64_t r = row0 + int64_t(j);
     if (p.b.table) {
@@ -361,6 +370,7 @@ __device__ __noinline__ void pr_plain_row(const PrArgs& p, int s, int row0, int 
   const auto score = [&](int j) {
     const T* k = at(p.k, p.k_stride, j);
     float d = 0.0f;
+#pragma unroll 1
     for (int i = 0; i < D; i += 2) {
       const float2 x = HalfOps<T>::unpack(*reinterpret_cast<const uint32_t*>(q + i));
       const float2 y = HalfOps<T>::unpack(*reinterpret_cast<const uint32_t*>(k + i));
@@ -370,26 +380,31 @@ __device__ __noinline__ void pr_plain_row(const PrArgs& p, int s, int row0, int 
     return d * p.a.scale_log2;
   };
   float m = -INFINITY;
+#pragma unroll 1
   for (int j = lo; j <= hi; ++j) m = fmaxf(m, score(j));
   const float ms = m == -INFINITY ? 0.0f : m;
-  for (int c = 0; c < D; c += 32) {
-    float o[32], l = 0.0f;
-    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 4) {
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+#pragma unroll 1
     for (int j = lo; j <= hi; ++j) {
       const float e = ex2(score(j) - ms);
-      const T* v = at(p.v, p.v_stride, j) + c;
+      const uint2 v = *reinterpret_cast<const uint2*>(at(p.v, p.v_stride, j) + c);
+      const float2 a = HalfOps<T>::unpack(v.x), b = HalfOps<T>::unpack(v.y);
       l += e;
-      for (int i = 0; i < 32; i += 2) {
-        const float2 y = HalfOps<T>::unpack(*reinterpret_cast<const uint32_t*>(v + i));
-        o[i] = fmaf(e, y.x, o[i]);
-        o[i + 1] = fmaf(e, y.y, o[i + 1]);
-      }
+      o.x = fmaf(e, a.x, o.x), o.y = fmaf(e, a.y, o.y), o.z = fmaf(e, b.x, o.z), o.w = fmaf(e, b.y, o.w);
+    }
+    if (part) {  // as a part's other rows lie
+      *reinterpret_cast<float4*>(out32 + c * 32) = o;
+      if (c == 0) *part = make_float2(m, l);
+      continue;
     }
     const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    for (int i = 0; i < 32; ++i) {
-      if (out32) out32[c + i] = o[i] * inv;
-      else out[c + i] = HalfOps<T>::from(o[i] * inv);
-    }
+    if (out32) *reinterpret_cast<float4*>(out32 + c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    else
+      *reinterpret_cast<uint2*>(out + c) =
+          make_uint2(HalfOps<T>::pack(o.x * inv, o.y * inv), HalfOps<T>::pack(o.z * inv, o.w * inv));
     if (c == 0 && lse) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
   }
 }
@@ -402,10 +417,19 @@ __device__ __forceinline__ bool pr_not_finite(uint32_t v) {
 
 // ---- the kernel ---------------------------------------------------------------------
 
-// An item as the scheduler hands it out; seq < 0: there is none left.
+// An item (or a part of one) as the scheduler hands it out; seq < 0: there is
+// none left.
 struct PrItem {
   int seq, head, tile;
+  int place, part, parts;  // place: of the launch; parts of the item's keys
   SeqSpan span;
+};
+
+// What hc_prompt_join_kernel needs of an item.
+struct PrJoin {
+  int parts;  // below 2: the item wrote its rows itself
+  int head, tile;
+  int row0, n;
 };
 
 // What every role derives from an item.
@@ -424,33 +448,41 @@ __device__ __forceinline__ PrGeom pr_geom(const PrItem& it, int group, int windo
   g.key_hi = min(it.span.len, p_last + 1);
   g.key0 = key_lo / PR_KEYS * PR_KEYS;
   g.units = g.key_hi > key_lo ? (g.key_hi - g.key0 + PR_KEYS - 1) / PR_KEYS : 0;
+  if (it.parts > 1) {
+    const int per = (g.units + it.parts - 1) / it.parts, first = it.part * per;
+    g.key0 += first * PR_KEYS;
+    g.units = max(0, min(per, g.units - first));
+    g.key_hi = min(g.key_hi, g.key0 + g.units * PR_KEYS);
+  } else if (it.part > 0) {
+    g.units = 0;
+  }
   return g;
 }
 
 template <class T, int D>
 __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
-    hc_prompt_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+    hc_prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                           const __grid_constant__ PrArgs p) {
   using Cfg = PrCfg<D>;
   constexpr int CG = Cfg::CG, ST = Cfg::kStages, SPAN = PR_ROWS * CG;
   constexpr uint32_t FMT = HalfOps<T>::kMap == CU_TENSOR_MAP_DATA_TYPE_FLOAT16 ? 0u : 1u;
   // the roles behind the softmax warps 0 .. 7; each is a warp of its own, since
   // what it does per tile is a chain of dependent steps
-  constexpr int LOAD_K = 8, LOAD_V = 9, ISSUER = 10, ISSUER_O = 11, SCHEDULER = 12, LOADERS = 4;
+  constexpr int LOAD_K = 8, LOAD_V = 9, ISSUER = 10, ISSUER_O = 11, ITEMS = 12, ITEM_WARPS = 4;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) uint4 clc_resp;
-  __shared__ __align__(8) uint64_t q_first, q_full, q_free, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], v_peer[ST];
-  __shared__ __align__(8) uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free, m_pass[4], l_pass[4];
-  __shared__ __align__(8) uint64_t item_full[2], item_empty[2], clc_full, clc_ready;
+  __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], v_peer[ST];
+  __shared__ __align__(8) uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free, m_pass[4], l_pass[4], l_free;
+  __shared__ __align__(8) uint64_t item_full[2], item_empty[2], clc_full, clc_ready, near_end;
   __shared__ PrItem s_items[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_odd[4];              // item number + 1 of a tile with a value that is not finite
   __shared__ float s_m[PR_ROWS];        // the rows' m after the last tile decided
-  __shared__ float2 s_l[2][2][PR_ROWS]; // [item parity] (m, l) of each warpgroup at an item's end
+  __shared__ float2 s_l[2][PR_ROWS];    // (m, l) of each warpgroup at an item's end
   const int t = int(threadIdx.x), warp = t >> 5, lane = t & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sq = base, sk = base + Cfg::kQ, sv = sk + ST * Cfg::kK, so = sv + ST * Cfg::kK;
+  const uint32_t sq = base, sk = base + Cfg::kQs * Cfg::kQ, sv = sk + ST * Cfg::kK, so = sv + ST * Cfg::kK;
   const int group = p.a.heads / p.a.kv_heads, window = p.a.window;
   int* const err = p.a.err;
   if (warp == ISSUER) {
@@ -463,9 +495,6 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     }
   }
   if (t == 0) {
-    mbar_init(&q_first, 8 * CG);
-    mbar_init(&q_full, LOADERS * CG);
-    mbar_init(&q_free, 1);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -474,20 +503,24 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       mbar_init(&v_peer[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], p.q_copy ? 1 : ITEM_WARPS * CG);
+      mbar_init(&q_free[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4 * CG);
       mbar_init(&p_ready[i], 4 * CG);
       mbar_init(&pv_done[i], 1);
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 15);  // every warp but the scheduler
+      mbar_init(&item_empty[i], 15);  // every warp but the one that finds them
     }
     for (int w = 0; w < 4; ++w) {
       mbar_init(&m_pass[w], 1);
       mbar_init(&l_pass[w], 2);
     }
-    mbar_init(&o_free, 8 * CG);
+    mbar_init(&o_free, ITEM_WARPS * CG);
+    mbar_init(&l_free, ITEM_WARPS);
     mbar_init(&clc_full, 1);
     mbar_init(&clc_ready, 1);
+    mbar_init(&near_end, 1);
     for (int i = 0; i < 4; ++i) s_odd[i] = 0;
   }
   tc_before();
@@ -495,6 +528,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   tc_after();
   const uint32_t tmem = s_tmem;
   pdl_wait_prior();
+  const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
   bool ok = true;
 
   // Item i of this CTA, read by every warp from the ring.
@@ -515,17 +549,18 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     const int x = rem + rr, tok = int((uint32_t(x) * inv_group) >> 21);
     return make_int2(tok0 + tok, x - tok * group);
   };
-  // The CTA's rows of an item into the swizzled operand layout by `n` threads: 16
-  // bytes at a time, neighbouring lanes neighbouring bytes of a row, all copies
+  // The CTA's rows of an item into the swizzled operand layout by `n` threads,
+  // where TMA cannot (a group that does not divide 128 rows, a negative
+  // scale): 16 bytes at a time, neighbouring lanes neighbouring bytes of a row, all copies
   // in flight together.  A negative scale flips Q's sign (so that the maximum
   // is that of the scores).
-  const auto load_q = [&](const PrItem& it, const PrGeom& g, int i0, int n) {
+  const auto load_q = [&](const PrItem& it, const PrGeom& g, uint32_t slot, int i0, int n) {
     const int rt = g.r0 + int(rank) * PR_ROWS;
     const int tok0 = rt / group, rem = rt - tok0 * group;
     const T* src = static_cast<const T*>(p.a.q) + int64_t(it.span.row0) * p.a.q_stride + it.head * group * D;
     const auto dst = [&](int i) {
       const int rr = i / (D / 8), c = i % (D / 8);
-      return sq + (c >> 3) * (PR_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+      return sq + slot * Cfg::kQ + (c >> 3) * (PR_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
     };
 #pragma unroll 4
     for (int i = i0; i < PR_ROWS * (D / 8); i += n) {
@@ -570,6 +605,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     PrItem it;
     int st = 0;
     uint32_t ph = 1;  // parity of the stage's last release; the first use waits for none
+    uint32_t nq = 0;  // items with tiles so far
     for (int n_it = 0; next_item(n_it, &it); ++n_it) {
       const PrGeom g = pr_geom(it, group, window, SPAN);
       const auto row_of = [&](int key) {
@@ -580,7 +616,30 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         return in ? int((int64_t(page) << p.b.page_shift) + (key & ((1 << p.b.page_shift) - 1))) : int(p.slots);
       };
       const int first = it.head * Cfg::kPieces + piece0;
+      if (!is_k && p.q_copy && g.units > 0) {
+        // Q: 128 (token, head of the group) rows from a token on, per 64 columns.
+        // Rows behind the sequence's last token are another's, or zeros;
+        // nothing of theirs is stored.
+        const uint32_t slot = nq % Cfg::kQs, use = nq / Cfg::kQs;
+        if (use > 0) ok = ok && pr_wait(&q_free[slot], (use - 1) & 1u, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (rank == 0 && elect_one()) mbar_expect_tx(&q_full[slot], Cfg::kQ * CG);
+        __syncwarp();
+        const int token = it.span.row0 + (g.r0 + int(rank) * PR_ROWS) / group;
+        const uint32_t bar = smem_u32(&q_full[slot]) & (CG == 2 ? kLeaderMask : 0xffffffffu);
+        if (elect_one())
+          for (int c = 0; c < Cfg::kPieces; ++c)
+            pr_tma_q<CG>(sq + slot * Cfg::kQ + c * (PR_ROWS * 128), &qmap, c, it.head * group, token, bar);
+        __syncwarp();
+        ++nq;
+      }
+      // the next item is asked for shortly before this one's last keys: earlier
+      // it would wait here while other CTAs run dry
+      const int ask = max(0, g.units - PR_AHEAD);
+      if (is_k && g.units == 0 && lane == 0) mbar_arrive(&near_end);
       for (int k0 = g.key0, i = 0; i < g.units; ++i, k0 += PR_KEYS) {
+        if (is_k && i == ask && lane == 0) mbar_arrive(&near_end);
         const int n = min(PR_KEYS, g.key_hi - k0);
         const auto copies = [&](int from) { return (min(keys, max(0, n - from)) + box - 1) >> shift; };
         const int c_n = copies(off);
@@ -612,6 +671,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     // after a timeout: the copies that nobody else waits for
     if (!ok && mine)
       for (int i = 0; i < ST; ++i) pr_wait(&full[i], ph, nullptr);
+    if (!ok && !is_k && rank == 0 && p.q_copy && nq > 0) pr_wait(&q_full[(nq - 1) % Cfg::kQs], (nq - 1) / Cfg::kQs & 1u, nullptr);
   } else if (warp == ISSUER || warp == ISSUER_O) {
     // ---- the products, issued by one thread of the pair's first CTA.  What
     // an issuer does between a barrier and its product is on every tile's path
@@ -624,14 +684,14 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     const auto issue_s = [&](bool last) {
       tc_after();
       if (elect_one()) {
-        const uint64_t a = pr_desc(sq, 16, 1024), b = pr_desc(sk + k_st * Cfg::kK, 16, 1024);
+        const uint64_t a = pr_desc(sq + nq % Cfg::kQs * Cfg::kQ, 16, 1024), b = pr_desc(sk + k_st * Cfg::kK, 16, 1024);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           pr_mma_ss<CG>(tmem + (sn & 1) * 128, a + ((k >> 2) * (PR_ROWS * 128) + (k & 3) * 32) / 16,
                         b + ((k >> 2) * (Cfg::kKeys * 128) + (k & 3) * 32) / 16, id_qk, k > 0);
         pr_commit<CG>(&s_full[sn & 1]);
         pr_commit<CG>(&k_empty[k_st]);
-        if (last) pr_commit<CG>(&q_free);
+        if (last) pr_commit<CG>(&q_free[nq % Cfg::kQs]);
       }
       __syncwarp();
       ++sn;
@@ -676,8 +736,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         continue;
       }
       if (warp == ISSUER) {
-        ok = ok && pr_wait(&q_full, nq & 1u, err);
-        if (nq == 0) ok = ok && pr_wait(&q_first, 0, err);
+        ok = ok && pr_wait(&q_full[nq % Cfg::kQs], nq / Cfg::kQs & 1u, err);
       }
       if constexpr (Cfg::kOwnP) {
         // S and O each by a warp of their own: all that orders them are the slots
@@ -724,20 +783,180 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       ++nq;
     }
   } else {
-    // ---- items: the sequences' tiles in order, each sequence's last rows
-    // (the longest sums) first, the KV heads of a tile side by side; and
-    // the Q of every item but the first
+    // ---- the items: which one is next, its Q, and the rows of the one before.
+    // The sequences' tiles in order, each sequence's last rows (the longest sums)
+    // first, the KV heads of a tile side by side.
+    const int w4 = warp - ITEMS;
     const auto tiles = [&](const SeqSpan& q) { return (q.n * group + SPAN - 1) / SPAN * p.a.kv_heads; };
-    int s0 = 0, before = 0;  // items of the sequences before s0
+    int s0 = 0, before = 0;  // places of the sequences before s0
+    SeqSpan own{};           // of the 32 sequences from `loaded` on, lane by lane
+    int loaded = -1, mine = 0, incl = 0;
+    // Key tiles of all items, about (every item of a sequence taken for its last),
+    // for an item's share: parts are as long as what a CTA gets when all get
+    // the same, so that few items over long keys fill the machine once.
+    int64_t all_units = 0;
+    if (p.split > 1) {
+      for (int s = lane; s < p.b.seqs; s += 32) {
+        bool bad;
+        const SeqSpan q = seq_span(p.b, s, &bad);
+        const int keys = window > 0 ? min(q.len, window + SPAN / group) : q.len;
+        all_units += int64_t(tiles(q)) * ((keys + PR_KEYS - 1) / PR_KEYS);
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) all_units += __shfl_xor_sync(0xffffffffu, all_units, d);
+    }
+    uint32_t nq = 0, v0 = 0, ends = 0;  // items with tiles whose Q was asked for; tiles and items with tiles that ended
+    // An item's rows, once its last product has landed: a lane has a row's sums.
+    const auto put_rows = [&](const PrItem& it, int n) {
+      const PrGeom g = pr_geom(it, group, window, SPAN);
+      if (it.part >= it.parts) return;  // no keys are left for this part
+      const int rt = g.r0 + int(rank) * PR_ROWS, tok0 = rt / group, rem = rt - tok0 * group, rr = w4 * 32 + lane;
+      const bool live = rt + rr < g.nrows;
+      float m = -INFINITY, l = 0.0f;
+      bool odd = false;
+      if (g.units > 0) {
+        v0 += uint32_t(g.units);
+        ok = ok && pr_wait(&l_pass[w4], ends & 1u, err);
+        ok = ok && pr_wait(&pv_done[(v0 - 1) & 1], ((v0 - 1) >> 1) & 1u, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        tc_after();
+        ++ends;
+        const float2 a = s_l[0][rr], b = s_l[1][rr];
+        m = fmaxf(a.x, b.x);
+        l = m == -INFINITY ? a.y + b.y : a.y * ex2((a.x - m) * sc) + b.y * ex2((b.x - m) * sc);
+        odd = *static_cast<volatile int*>(&s_odd[n & 3]) == n + 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_free);
+      }
+      const uint32_t oa = tmem + (uint32_t(w4) * 32u << 16) + Cfg::kTmemO;
+      const auto done_with_o = [&] {  // the next item's first product may overwrite O
+        if (g.units == 0) return;
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader<CG>(&o_free);
+      };
+      if (it.parts > 1) {
+        // a part leaves its sums undivided: [warp's 32 rows][head_dim / 4][row] float4
+        const int64_t rows = int64_t(it.place) * SPAN + int(rank) * PR_ROWS + w4 * 32;
+        float* const to = p.part_o + rows * D + lane * 4;
+        if (!odd) {
+          p.part_ml[rows + lane] = make_float2(m * sc, l);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tm_ld16(oa + c, o);
+            tm_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(to + (c + e) * 32) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      } else if (!odd) {
+        const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+        const int64_t tok = int64_t(it.span.row0 + tok0) * p.a.heads + it.head * group;
+        if (live && p.a.lse) {
+          const int2 own = row_at(0, rem, rr);
+          p.a.lse[tok + own.x * p.a.heads + own.y] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
+        }
+        // RB bytes of each of the warp's 32 rows at a time through shared memory,
+        // so that neighbouring lanes store neighbouring bytes: 16-byte chunk c of
+        // row r lies at chunk c ^ key(r)
+        constexpr int RB = Cfg::kRowBytes, CH = RB / 16, STEP = 32 / CH;  // rows of one pass of the stores
+        const uint32_t stage = so + uint32_t(w4) * (32 * RB);
+        const auto key = [](int r) { return CH == 4 ? (r >> 1) & 3 : r & 7; };
+        const auto put = [&](int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * RB + ((c ^ key(lane)) << 4)), "r"(a),
+                       "r"(b), "r"(d), "r"(e)
+                       : "memory");
+        };
+        const int esz = p.a.out_f32 ? 4 : 2;
+        uint8_t* const out = static_cast<uint8_t*>(p.a.out) + tok * D * esz + lane % CH * 16;
+        const auto flush = [&](int bytes) {  // the staged bytes start there in a row
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 32; i += STEP) {
+            const int r = i + lane / CH;
+            const int2 w = row_at(0, rem, w4 * 32 + r);
+            uint4 x;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                         : "r"(stage + r * RB + ((lane % CH ^ key(r)) << 4))
+                         : "memory");
+            if (rt + w4 * 32 + r < g.nrows)
+              *reinterpret_cast<uint4*>(out + int64_t((w.x * p.a.heads + w.y) * D * esz + bytes)) = x;
+          }
+          __syncwarp();
+        };
+        const int cols = RB / esz;  // of a pass: a multiple of 16
+#pragma unroll 1
+        for (int c = 0; c < D; c += cols) {
+#pragma unroll 1
+          for (int h = 0; h < cols; h += 16) {
+            uint32_t o[16];
+            if (g.units > 0) {
+              tm_ld16(oa + c + h, o);
+              tm_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+            if (p.a.out_f32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) put(h / 4 + e, o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  w[i] = HalfOps<T>::pack(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
+                put(h / 8 + e, w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+          if (c + cols == D) done_with_o();
+          flush(c * esz);
+        }
+      }
+      if (it.parts > 1 || odd) done_with_o();
+      if (odd && (live || it.parts > 1)) {
+        const int2 own = row_at(tok0, rem, live ? rr : 0);
+        const int pos = g.pos0 + own.x, lim = live ? min(pos, it.span.len - 1) : -1;
+        const int low = window > 0 ? max(0, pos - window + 1) : 0;
+        const T* q = static_cast<const T*>(p.a.q) + int64_t(it.span.row0 + own.x) * p.a.q_stride + (it.head * group + own.y) * D;
+        const int64_t row = int64_t(it.span.row0 + own.x) * p.a.heads + it.head * group + own.y;
+        const int64_t rows = int64_t(it.place) * SPAN + int(rank) * PR_ROWS + w4 * 32;
+        const bool part = it.parts > 1;
+        pr_plain_row<T, D>(p, it.seq, it.span.row0, it.head, q, part ? max(low, g.key0) : low,
+                           part ? min(lim, g.key_hi - 1) : lim, static_cast<T*>(p.a.out) + row * D,
+                           part ? p.part_o + rows * D + lane * 4
+                                : p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr,
+                           p.a.lse ? p.a.lse + row : nullptr, part ? p.part_ml + rows + lane : nullptr);
+      }
+      __syncwarp();
+    };
     int x = int(blockIdx.x) / CG;
-    int nq = 0;
-    const int loader = t - 32 * SCHEDULER;
+    PrItem prev;
     for (int n_it = 0; ok; ++n_it) {
       PrItem it;
       it.seq = -1;
-      if (warp == SCHEDULER) {
+      if (warp == ITEMS) {
         if (n_it > 0) {
-          // the answer to the request made when the last item went out
+          // a pair's first CTA asks for both, once the other has read the last answer
+          if (lane == 0) {
+            mbar_expect_tx(&clc_full, 16);
+            if (CG == 2 && rank == 1) arrive_leader<CG>(&clc_ready);
+            if (rank == 0) {
+              ok = pr_wait(&near_end, uint32_t(n_it - 1) & 1u, err);
+              if (CG == 2) ok = ok && pr_wait(&clc_ready, uint32_t(n_it - 1) & 1u, err);
+              if (ok) clc_ask<CG>(&clc_resp, &clc_full);
+            }
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           ok = pr_wait(&clc_full, uint32_t(n_it - 1) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
@@ -746,29 +965,48 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           x = first < 0 ? -1 : first / CG;
           __syncwarp();
         }
-        if (x < before) s0 = before = 0;  // items come in launch order, but nothing promises it
-        while (x >= 0 && s0 < p.b.seqs) {  // 32 sequences at a time
-          SeqSpan own{};
-          bool bad = false;
-          if (s0 + lane < p.b.seqs) own = seq_span(p.b, s0 + lane, &bad);
-          if (bad && err) atomicExch(err, DEVICE_ERR_PAGE);
-          const int mine = tiles(own);
-          int incl = mine;
+        // first parts first, so that whole items start at once
+        const int part = p.split > 1 && x >= 0 ? x / p.items : 0, y = x - part * p.items;
+        if (y < before) s0 = before = 0, loaded = -1;
+        while (y >= 0 && s0 < p.b.seqs) {  // 32 sequences at a time
+          if (loaded != s0) {
+            loaded = s0;
+            own = SeqSpan{};
+            bool bad = false;
+            if (s0 + lane < p.b.seqs) own = seq_span(p.b, s0 + lane, &bad);
+            if (bad && err) atomicExch(err, DEVICE_ERR_PAGE);
+            mine = incl = tiles(own);
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += v;
+            for (int d = 1; d < 32; d <<= 1) {
+              const int v = __shfl_up_sync(0xffffffffu, incl, d);
+              if (lane >= d) incl += v;
+            }
           }
-          const unsigned hit = __ballot_sync(0xffffffffu, x < before + incl);
+          const unsigned hit = __ballot_sync(0xffffffffu, y < before + incl);
           if (hit) {
             const int w = __ffs(hit) - 1;
-            const int at = x - before - __shfl_sync(0xffffffffu, incl - mine, w), n = __shfl_sync(0xffffffffu, mine, w);
+            const int at = y - before - __shfl_sync(0xffffffffu, incl - mine, w), n = __shfl_sync(0xffffffffu, mine, w);
             it.span.row0 = __shfl_sync(0xffffffffu, own.row0, w);
             it.span.n = __shfl_sync(0xffffffffu, own.n, w);
             it.span.len = __shfl_sync(0xffffffffu, own.len, w);
             it.seq = s0 + w;
-            it.head = at % p.a.kv_heads;
-            it.tile = n / p.a.kv_heads - 1 - at / p.a.kv_heads;
+            it.place = x;
+            it.part = part;
+            it.parts = 1;
+            it.tile = at / p.a.kv_heads;
+            it.head = at - it.tile * p.a.kv_heads;
+            it.tile = n / p.a.kv_heads - 1 - it.tile;
+            if (p.split > 1) {
+              PrItem whole = it;
+              whole.part = 0;
+              const int units = pr_geom(whole, group, window, SPAN).units;
+              const int64_t share = all_units > 0 ? int64_t(units) * p.workers / all_units : 1;
+              const int parts = int(min(share, int64_t(min(p.split, units / PR_PART))));
+              if (parts > 1) {
+                const int per = (units + parts - 1) / parts;
+                it.parts = (units + per - 1) / per;
+              }
+            }
             break;
           }
           before += __shfl_sync(0xffffffffu, incl, 31);
@@ -780,34 +1018,37 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           if (!ok) break;
         }
         if (lane == 0) {
+          if (p.split > 1 && rank == 0 && part == 0 && y >= 0) {
+            PrJoin j{};
+            if (it.seq >= 0) j = {it.parts, it.head, it.tile, it.span.row0, it.span.n};
+            p.join[y] = j;
+          }
           s_items[n_it & 1] = it;
           mbar_arrive(&item_full[n_it & 1]);
-          if (it.seq >= 0) {
-            // a pair's first CTA asks for both, once the other has read the last answer
-            mbar_expect_tx(&clc_full, 16);
-            if (CG == 2 && rank == 1) arrive_leader<CG>(&clc_ready);
-            if (rank == 0) {
-              if (CG == 2) ok = pr_wait(&clc_ready, uint32_t(n_it) & 1u, err);
-              if (ok) clc_ask<CG>(&clc_resp, &clc_full);
-            }
-          }
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok || it.seq < 0) break;
-      } else if (!next_item(n_it, &it)) {
-        break;
+        __syncwarp();
+      } else {
+        next_item(n_it, &it);
       }
-      const PrGeom g = pr_geom(it, group, window, SPAN);
-      if (g.units > 0) {
-        if (n_it > 0) {
-          if (nq > 0) ok = pr_wait(&q_free, uint32_t(nq - 1) & 1u, err);
+      if (!ok) break;
+      if (!p.q_copy && it.seq >= 0) {
+        const PrGeom g = pr_geom(it, group, window, SPAN);
+        if (g.units > 0) {
+          const uint32_t slot = nq % Cfg::kQs, use = nq / Cfg::kQs;
+          if (use > 0) ok = pr_wait(&q_free[slot], (use - 1) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          load_q(it, g, loader, 32 * LOADERS);
+          load_q(it, g, slot, t - 32 * ITEMS, 32 * ITEM_WARPS);
+          if (lane == 0) arrive_leader<CG>(&q_full[slot]);
+          ++nq;
         }
-        if (lane == 0) arrive_leader<CG>(&q_full);
-        ++nq;
       }
+      if (n_it > 0) {
+        put_rows(prev, n_it - 1);
+        if (!ok) break;
+      }
+      if (it.seq < 0) break;
+      prev = it;
     }
   }
   } else {
@@ -816,7 +1057,6 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     // of its parity (over all items)
     const int wg = warp >> 2, w4 = warp & 3, lt = t & 127;
     const uint32_t lanes = uint32_t(w4) * 32u << 16;
-    const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
     uint32_t v0 = 0;    // tiles before this item
     uint32_t ends = 0;  // items with tiles so far
     const uint32_t sa = tmem + lanes + uint32_t(wg) * 128, pa = tmem + lanes + Cfg::p_col(uint32_t(wg));
@@ -827,18 +1067,14 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       const int rt = g.r0 + int(rank) * PR_ROWS;  // the CTA's first row
       const int tok0 = rt / group, rem = rt - tok0 * group;
       const bool live = rt + lt < g.nrows;
-      if (n_it == 0) {
-        if (g.units > 0) load_q(it, g, t, 256);
-        if (lane == 0) arrive_leader<CG>(&q_first);
-      }
       const int2 own = row_at(tok0, rem, live ? lt : 0);  // token, head of the group
       const int pos = g.pos0 + own.x;
       const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
+      float m = -INFINITY, l = 0.0f;
       // keys [all_lo, all_hi] are seen by every row of the item (in a pair
       // each CTA looks after half of every value for both)
       const int all_hi = min(it.span.len - 1, g.pos0 + g.r0 / group);
       const int all_lo = window > 0 ? g.pos0 + (min(g.r0 + SPAN, g.nrows) - 1) / group - window + 1 : 0;
-      float m = -INFINITY, l = 0.0f;
       for (int u = int((v0 ^ uint32_t(wg)) & 1u); u < g.units; u += 2) {
         const uint32_t v = v0 + uint32_t(u);
         const int k0 = g.key0 + u * PR_KEYS;
@@ -848,12 +1084,11 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         uint32_t s[PR_KEYS];
 #pragma unroll
         for (int c = 0; c < PR_KEYS; c += 32) tm_ld32(sa + c, s + c);
-        // meanwhile: m as the other warpgroup left it at the tile before
+        // meanwhile: m as the other warpgroup left it at the tile before (an
+        // item's first tile only waits its turn: s_m is the last item's until then)
         float prev = -INFINITY;
-        if (u > 0) {
-          ok = ok && pr_wait(&m_pass[w4], (v - 1) & 1u, err);
-          prev = *static_cast<volatile float*>(&s_m[lt]);
-        }
+        if (v > 0) ok = ok && pr_wait(&m_pass[w4], (v - 1) & 1u, err);
+        if (u > 0) prev = *static_cast<volatile float*>(&s_m[lt]);
         __syncwarp();
         tm_wait_ld();
         if constexpr (Cfg::kOwnP) {
@@ -866,7 +1101,12 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           const int hi = lim - k0, lo = low - k0;
 #pragma unroll
           for (int c = 0; c < PR_KEYS; ++c)
-            if (c > hi || c < lo) s[c] = 0xff800000u;
+            if (c > hi) s[c] = 0xff800000u;
+          if (k0 < all_lo) {
+#pragma unroll
+            for (int c = 0; c < PR_KEYS; ++c)
+              if (c < lo) s[c] = 0xff800000u;
+          }
         }
         float mx[4];
 #pragma unroll
@@ -908,60 +1148,58 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         const float ms = m == -INFINITY ? 0.0f : m * sc;
         const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(-ms, -ms);
         uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-        const auto exps = [&](auto poly) {
 #pragma unroll
-          for (int b = 0; b < PR_KEYS; b += 32) {
-            uint32_t pk[16];
+        for (int b = 0; b < PR_KEYS; b += 32) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              const uint64_t x = fma2(pack2(__uint_as_float(s[b + c]), __uint_as_float(s[b + c + 1])), sc2, nm2);
-              float e0, e1;
-              if (poly.value && (c >> 1) % PR_POLY_EVERY == PR_POLY_EVERY - 1) {
-                ex2_poly2(x, e0, e1);
-              } else {
-                unpack2(x, e0, e1);
-                e0 = ex2(e0), e1 = ex2(e1);
-              }
-              sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(e0, e1));
-              pk[c >> 1] = HalfOps<T>::pack(e0, e1);
-            }
-            if (Cfg::kOwnP && b == 0) {  // the P slot: the product that read it last
-              if (v >= 2) ok = ok && pr_wait(&pv_done[wg], ((v >> 1) - 1) & 1u, err);
-              __syncwarp();
-              tc_after();
-            }
-            tm_st16(pa + b / 2, pk);
+          for (int c = 0; c < 32; c += 2) {
+            float e0, e1;
+            unpack2(fma2(pack2(__uint_as_float(s[b + c]), __uint_as_float(s[b + c + 1])), sc2, nm2), e0, e1);
+            e0 = ex2(e0), e1 = ex2(e1);
+            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(e0, e1));
+            pk[c >> 1] = HalfOps<T>::pack(e0, e1);
           }
-        };
-        if (edge) exps(std::false_type{});  // -inf has to give 0
-        else exps(std::true_type{});
+          if (Cfg::kOwnP && b == 0) {  // the P slot: the product that read it last
+            if (v >= 2) ok = ok && pr_wait(&pv_done[wg], ((v >> 1) - 1) & 1u, err);
+            __syncwarp();
+            tc_after();
+          }
+          tm_st16(pa + b / 2, pk);
+        }
         {
           float a, b;
           unpack2(add2(sum[0], sum[1]), a, b);
           l += a + b;
         }
         if (edge) {
-          // values of keys that no row uses, and values that only some rows see
+          // values that only some rows see are looked through for what is not
+          // finite; values behind the last key in use become 0 up to the next
+          // 16 (the product goes no further)
+          constexpr int CH = Cfg::kPiecesV * 8;  // 16-byte chunks of a key's values in this CTA
           const uint32_t st = v % ST, vt = sv + st * Cfg::kK;
+          const int used = min(PR_KEYS, g.key_hi - k0), seen = k0 < all_lo ? 0 : max(0, all_hi + 1 - k0);
+          const auto chunk = [&](int i) {
+            return vt + (i % CH >> 3) * (PR_KEYS * 128) + i / CH * 128 + ((i & 7) << 4);
+          };
           ok = ok && pr_wait(&v_full[st], (v / ST) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
           bool odd = false;
-          if (ok)
-            for (int i = lt; i < PR_KEYS * Cfg::kPiecesV * 8; i += 128) {
-              const int key = i / (Cfg::kPiecesV * 8), c = i % (Cfg::kPiecesV * 8);
-              const uint32_t at = vt + (c >> 3) * (PR_KEYS * 128) + key * 128 + ((c & 7) << 4);
-              if (k0 + key >= g.key_hi) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-              } else {
-                uint32_t a, b, d, e;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(a), "=r"(b), "=r"(d), "=r"(e)
-                             : "r"(at)
-                             : "memory");
-                odd = odd || pr_not_finite<T>(a) || pr_not_finite<T>(b) || pr_not_finite<T>(d) || pr_not_finite<T>(e);
-              }
+          if (ok) {
+#pragma unroll 4
+            for (int i = seen * CH + lt; i < used * CH; i += 128) {
+              uint32_t a, b, d, e;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(a), "=r"(b), "=r"(d), "=r"(e)
+                           : "r"(chunk(i))
+                           : "memory");
+              odd = odd || pr_not_finite<T>(a) || pr_not_finite<T>(b) || pr_not_finite<T>(d) || pr_not_finite<T>(e);
             }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (used & 15) {
+              for (int i = used * CH + lt; i < (used + 15 & ~15) * CH; i += 128)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk(i)), "r"(0u) : "memory");
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+          }
           if (__any_sync(0xffffffffu, odd) && lane == 0) {
             // both CTAs' rows are the sums of both CTAs' dims
             for (int c = 0; c < CG; ++c) {
@@ -975,8 +1213,8 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
                     : "memory");
             }
           }
-          // what was written here is read by the pair's products
-          if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          // what was written here is read by the pair's products, and its flag by the other CTA
+          if (CG == 2 && ((used & 15) || __any_sync(0xffffffffu, odd))) asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
         tm_wait_st();
         tc_before();
@@ -984,107 +1222,16 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         if (lane == 0 && ok) arrive_leader<CG>(&p_ready[wg]);
       }
       v0 += uint32_t(g.units);
-      // ---- the rows' outputs: both warpgroups' sums, and O once the last
-      // product has landed (the one two before it has: its slot was used again)
+      // ---- the item's sums of this warpgroup's tiles go to the item warps
       if (g.units > 0) {
-        s_l[ends & 1][wg][lt] = make_float2(m, l);
+        if (ends > 0) ok = ok && pr_wait(&l_free, (ends - 1) & 1u, err);
+        s_l[wg][lt] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&l_pass[w4]);
-        ok = ok && pr_wait(&l_pass[w4], ends & 1u, err);
-        __syncwarp();
-        const float2 a = s_l[ends & 1][0][lt], b = s_l[ends & 1][1][lt];
-        m = fmaxf(a.x, b.x);
-        l = m == -INFINITY ? a.y + b.y : a.y * ex2((a.x - m) * sc) + b.y * ex2((b.x - m) * sc);
-        ok = ok && pr_wait(&pv_done[(v0 - 1) & 1], ((v0 - 1) >> 1) & 1u, err);
-        __syncwarp();
-        tc_after();
         ++ends;
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-      const int64_t row = int64_t(it.span.row0 + own.x) * p.a.heads + it.head * group + own.y;
-      float* lse = p.a.lse ? p.a.lse + row : nullptr;
-      const bool odd = g.units > 0 && *static_cast<volatile int*>(&s_odd[n_it & 3]) == n_it + 1;
-      if (live && lse && wg == 0 && !odd) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m * sc + log2f(l));
-      // 64 bytes of each of the warp's 32 rows at a time through shared
-      // memory, so that four lanes store 64 consecutive bytes: 16-byte chunk c of
-      // row r at chunk c ^ (r / 2 % 4)
-      const uint32_t stage = so + uint32_t(warp) * 2048;
-      const auto put = [&](int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)), "r"(a),
-                     "r"(b), "r"(d), "r"(e)
-                     : "memory");
-      };
-      const int esz = p.a.out_f32 ? 4 : 2;
-      uint8_t* dst[4];  // this lane's 16 bytes of four rows, column 0; nullptr: no row
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rr = w4 * 32 + i * 8 + (lane >> 2);
-        const int2 w = row_at(tok0, rem, rr);
-        const int64_t at = (int64_t(it.span.row0 + w.x) * p.a.heads + it.head * group + w.y) * D;
-        dst[i] = rt + rr < g.nrows && !odd ? static_cast<uint8_t*>(p.a.out) + at * esz + (lane & 3) * 16 : nullptr;
-      }
-      const auto flush = [&](int col) {  // the staged bytes start at column col
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = i * 8 + (lane >> 2), c = lane & 3;
-          uint4 x;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                       : "r"(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4))
-                       : "memory");
-          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + col * esz) = x;
-        }
-        __syncwarp();
-      };
-#pragma unroll 1
-      for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
-        uint32_t o[32];
-        if (g.units > 0) {
-          tm_ld32(oa + c, o);
-          tm_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
-        if (p.a.out_f32) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              put(e, o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
-            flush(c + 16 * h);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = HalfOps<T>::pack(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
-            put(e, w[0], w[1], w[2], w[3]);
-          }
-          flush(c);
-        }
-      }
-      if (g.units > 0) {  // the next item's first product may overwrite O
-        tc_before();
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(&o_free);
-      }
-      if (odd) {
-        if (live && wg == 0)
-          pr_plain_row<T, D>(p, it.seq, it.span.row0, it.head,
-                             static_cast<const T*>(p.a.q) + int64_t(it.span.row0 + own.x) * p.a.q_stride +
-                                 (it.head * group + own.y) * D,
-                             max(low, 0), lim, static_cast<T*>(p.a.out) + row * D,
-                             p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr, lse);
-        __syncwarp();
-      }
     }
     // after a timeout the products in flight get one more bounded wait before
     // the tensor memory is freed
@@ -1103,8 +1250,64 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   }
 }
 
+// Joins the parts of an item's keys: a warp takes 32 rows, a thread each, and
+// 32 of their columns (a multiple of 32 for every head_dim): the maximum of
+// all parts, then the sums against it in the parts' order.
+constexpr int PJ_THREADS = 256;
 template <class T, int D>
-cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, cudaStream_t st) {
+__global__ void __launch_bounds__(PJ_THREADS) hc_prompt_join_kernel(const __grid_constant__ PrArgs p) {
+  constexpr int SPAN = PR_ROWS * PrCfg<D>::CG, COLS = 32;
+  pdl_wait_prior();
+  const int lane = int(threadIdx.x) & 31, unit = int(blockIdx.y) * (PJ_THREADS / 32) + (int(threadIdx.x) >> 5);
+  const PrJoin it = p.join[blockIdx.x];
+  if (it.parts < 2) return;
+  const int group = p.a.heads / p.a.kv_heads;
+  const int r32 = unit / (D / COLS) * 32, col = unit % (D / COLS) * COLS;
+  const int x = it.tile * SPAN + r32 + lane;
+  if (x >= it.n * group) return;
+  const int64_t rows = int64_t(blockIdx.x) * SPAN + r32, step = int64_t(p.items) * SPAN;
+  const float2* ml = p.part_ml + rows + lane;
+  const float* po = p.part_o + rows * D + col * 32 + lane * 4;
+  float mx = -INFINITY;
+  for (int i = 0; i < it.parts; ++i) mx = fmaxf(mx, ml[i * step].x);
+  const float ms = mx == -INFINITY ? 0.0f : mx;
+  float o[COLS], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < COLS; ++e) o[e] = 0.0f;
+  for (int i = 0; i < it.parts; ++i) {
+    const float2 s = ml[i * step];
+    const float f = ex2(s.x - ms);
+    sum += f * s.y;
+#pragma unroll
+    for (int e = 0; e < COLS; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(po + i * step * D + e * 32);
+      o[e] += f * v.x, o[e + 1] += f * v.y, o[e + 2] += f * v.z, o[e + 3] += f * v.w;
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  const int64_t row = int64_t(it.row0 + x / group) * p.a.heads + it.head * group + x % group;
+  if (p.a.out_f32) {
+    float* to = static_cast<float*>(p.a.out) + row * D + col;
+#pragma unroll
+    for (int e = 0; e < COLS; e += 4)
+      *reinterpret_cast<float4*>(to + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+  } else {
+    T* to = static_cast<T*>(p.a.out) + row * D + col;
+#pragma unroll
+    for (int e = 0; e < COLS; e += 8)
+      *reinterpret_cast<uint4*>(to + e) =
+          make_uint4(HalfOps<T>::pack(o[e] * inv, o[e + 1] * inv), HalfOps<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
+                     HalfOps<T>::pack(o[e + 4] * inv, o[e + 5] * inv), HalfOps<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+  }
+  if (col == 0 && p.a.lse) p.a.lse[row] = sum == 0.0f ? -INFINITY : 0.6931471805599453f * (mx + log2f(sum));
+}
+
+constexpr int kPrMaxSms = 160;  // that the workspace allows for
+constexpr size_t pr_places(int sms, int dim) { return size_t(sms / (dim == 64 ? 1 : 2) * PR_PLACES); }
+constexpr size_t pr_span(int dim) { return dim == 64 ? PR_ROWS : 2 * PR_ROWS; }
+
+template <class T, int D>
+cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, void* workspace, cudaStream_t st) {
   using Cfg = PrCfg<D>;
   auto kernel = hc_prompt_attn_kernel<T, D>;
   static std::atomic<uint64_t> attr{0};
@@ -1118,20 +1321,38 @@ cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, cudaStream_t st) {
   p.whole_k = bk == Cfg::kKeys, p.whole_v = bv == PR_KEYS;
   p.box_v = __builtin_ctz(bv);
   p.slots = int64_t(kv.slots);
-  CUtensorMap km, vm;
+  const int group = p.a.heads / p.a.kv_heads;
+  CUtensorMap qm{}, km, vm;
   e = encode_kv_map(&km, HalfOps<T>::kMap, kv.k, kv.slots, kv.k_stride, p.a.kv_heads, D, bk,
                              p.whole_k ? Cfg::kPieces : 1);
   if (e == cudaSuccess)
     e = encode_kv_map(&vm, HalfOps<T>::kMap, kv.v, kv.slots, kv.v_stride, p.a.kv_heads, D, bv, p.whole_v ? Cfg::kPiecesV : 1);
   if (e != cudaSuccess) return e;
+  p.q_copy = PR_ROWS % group == 0 && p.a.scale_log2 >= 0.0f;
+  if (p.q_copy) {
+    const cuuint64_t dims[4] = {64, D / 64, cuuint64_t(p.a.heads), cuuint64_t(p.b.rows)};
+    const cuuint64_t strides[3] = {128, D * 2, cuuint64_t(p.a.q_stride) * 2};
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(group), cuuint32_t(PR_ROWS / group)};
+    e = encode_map(&qm, HalfOps<T>::kMap, 4, p.a.q, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
   // every sequence adds at most one tile to those of the rows put together
   constexpr int SPAN = PR_ROWS * Cfg::CG;
-  const int group = p.a.heads / p.a.kv_heads;
   const int64_t items =
       (int64_t(p.b.rows) * group / SPAN + std::min(p.b.seqs, p.b.rows)) * p.a.kv_heads;
   if (items * Cfg::CG > INT32_MAX) return cudaErrorInvalidValue;
+  p.items = int(items);
+  // Few items over long keys are cut into parts, as far as the workspace goes
+  p.workers = sm_count() / Cfg::CG;
+  const size_t places = pr_places(std::min(kPrMaxSms, sm_count()), D);
+  const int64_t keys = p.b.table ? int64_t(p.b.width) << p.b.page_shift : p.a.max_q;
+  const int64_t seen = p.a.window > 0 ? std::min(keys, int64_t(p.a.window) + SPAN / group + PR_KEYS) : keys;
+  p.split = int(std::max<int64_t>(1, std::min(int64_t(places) / items, (seen + PR_KEYS - 1) / PR_KEYS / PR_PART)));
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + places * SPAN * D);
+  p.join = reinterpret_cast<PrJoin*>(p.part_ml + places * SPAN);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(items * Cfg::CG));
+  cfg.gridDim = dim3(unsigned(items * p.split * Cfg::CG));
   cfg.blockDim = dim3(Cfg::kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = st;
@@ -1144,21 +1365,29 @@ cudaError_t launch_prompt(PrArgs& p, const KvSource& kv, cudaStream_t st) {
   at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, km, vm, p);
+  e = cudaLaunchKernelEx(&cfg, kernel, qm, km, vm, p);
+  if (e != cudaSuccess || p.split == 1) return e;
+  return launch_pdl(hc_prompt_join_kernel<T, D>, dim3(unsigned(items), SPAN / 32 * (D / 32) / (PJ_THREADS / 32)), dim3(PJ_THREADS), 0, st, p);
 }
 
 template <class T>
-cudaError_t launch_prompt_t(PrArgs& p, const KvSource& kv, cudaStream_t st) {
+cudaError_t launch_prompt_t(PrArgs& p, const KvSource& kv, void* ws, cudaStream_t st) {
   switch (p.a.dim) {
-    case 64: return launch_prompt<T, 64>(p, kv, st);
-    case 128: return launch_prompt<T, 128>(p, kv, st);
-    default: return launch_prompt<T, 256>(p, kv, st);
+    case 64: return launch_prompt<T, 64>(p, kv, ws, st);
+    case 128: return launch_prompt<T, 128>(p, kv, ws, st);
+    default: return launch_prompt<T, 256>(p, kv, ws, st);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, cudaStream_t st) {
+size_t attn_prompt_workspace_bytes(int dim) {
+  const size_t places = pr_places(kPrMaxSms, dim);
+  return places * pr_span(dim) * (size_t(dim) * 4 + 8) + places / 2 * sizeof(PrJoin);
+}
+
+cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvSource& kv, void* workspace,
+                               cudaStream_t st) {
   PrArgs p{};
   p.a = a;
   p.b = b;
@@ -1166,7 +1395,8 @@ cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvS
   p.v = kv.v;
   p.k_stride = int64_t(kv.k_stride);
   p.v_stride = int64_t(kv.v_stride);
-  return kv.dtype == HPC_DTYPE_F16 ? launch_prompt_t<__half>(p, kv, st) : launch_prompt_t<__nv_bfloat16>(p, kv, st);
+  return kv.dtype == HPC_DTYPE_F16 ? launch_prompt_t<__half>(p, kv, workspace, st)
+                                   : launch_prompt_t<__nv_bfloat16>(p, kv, workspace, st);
 }
 
 }  // namespace hc
