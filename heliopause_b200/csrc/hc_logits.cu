@@ -17,13 +17,14 @@
 // can still be among its k best; a second launch joins the chunks of each row.
 //   - The first 4096 give a floor without a sort: the k-th largest of 128 group
 //     maxima is reached by at least k tokens and by few others.  It is raised
-//     from the kept keys after two and four steps, so that most later steps end
+//     from the kept keys after two more steps, so that most later steps end
 //     with one comparison per warp.
 //   - Tokens of the history or with a bias (hundreds of a chunk's 32768) are left
 //     out of the stream and taken from a list of their own, one thread each: in
 //     the stream every warp that met one stood through its f64 division (the
 //     64 x 262144 batch then took 77 us).
-//   - Past the first step the mask is looked up for tokens above the floor only.
+//   - The chunk's mask waits in shared memory: looked up in place, for the tokens
+//     above the floor only, it held every warp up for two or three reads a step.
 //   - The survivors get such a floor once more and are ranked by counting.
 // Keys are (ordered value, complement of the id): no two are equal, so the
 // result does not depend on any order of execution.  The chunk's part of the
@@ -46,6 +47,7 @@ constexpr int LG_MAX_STEPS = 8;
 constexpr int LG_GROUPS = 128;
 constexpr int LG_MAX_K = 64;
 constexpr int LG_BIASES = 512;                 // of a chunk, kept in shared memory
+constexpr int LG_RANKED = 256;                   // kept keys that are ranked as they are (a floor first costs 2 us)
 constexpr int LG_CAND = 2560;                  // kept keys
 constexpr int LG_FLAGS = 4096;                 // listed tokens with a history or a bias
 // a token's 16 bits: seen in the history, has a bias, times in the output
@@ -125,6 +127,7 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
   __shared__ uint16_t s_flag[TOUCHED ? LG_FLAGS : 1];
   __shared__ int b_id[TOUCHED ? LG_BIASES : 1];
   __shared__ float b_val[TOUCHED ? LG_BIASES : 1];
+  __shared__ uint32_t s_allow[MASK ? LG_STEP * LG_MAX_STEPS / 32 : 1];
   __shared__ uint64_t s_floor, s_best[LG_THREADS / 32];
   __shared__ float s_over;
   __shared__ int s_n, s_flags, s_biases;
@@ -160,6 +163,10 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
   };
   float x[LG_EPT];
   load(0, x);
+  if constexpr (MASK) {
+    const uint32_t* allow = p.allowed + int64_t(row) * p.allowed_stride + c0 / 32;
+    for (int i = t; i < (n + 31) / 32; i += LG_THREADS) s_allow[i] = allow[i];
+  }
   double rep = 1.0, freq = 0.0, pres = 0.0;
   int64_t hist_a = 0, hist_b = 0, out0 = 0, bias_a = 0, bias_b = 0;
   if (TOUCHED && p.hist) {
@@ -183,35 +190,36 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
         if (at < LG_FLAGS) s_flag[at] = uint16_t(o);
       }
     };
+    // one warp picks out the chunk's biases, in list order; the others count the history
+    const bool biased = bias_b > bias_a;
+    const int lane = t & 31, counters = biased ? LG_THREADS - 32 : LG_THREADS;
 #pragma unroll 4
-    for (int64_t h = hist_a + t; h < hist_b; h += LG_THREADS) {
+    for (int64_t h = t < counters ? hist_a + t : hist_b; h < hist_b; h += counters) {
       const uint32_t o = uint32_t(p.hist[h]) - uint32_t(c0);  // (a negative id wraps past every chunk)
       if (o < uint32_t(n)) {
         flag(o, LG_SEEN);
         if (counted && h >= out0) atomicAdd(&cnt[o >> 1], 1u << (16 * (o & 1)));
       }
     }
-    if (t < 32 && bias_b > bias_a) {
-      // one warp picks out the chunk's biases, in list order
+    if (t >= counters) {
       int kept = 0;
       for (int64_t h0 = bias_a; h0 < bias_b; h0 += 32) {
-        const int64_t h = h0 + t;
+        const int64_t h = h0 + lane;
         const uint32_t o = h < bias_b ? uint32_t(p.bias_ids[h]) - uint32_t(c0) : 0xffffffffu;
         const bool in = o < uint32_t(n);
         const unsigned m = __ballot_sync(0xffffffffu, in);
-        const int at = kept + __popc(m & ((1u << t) - 1u));
+        const int at = kept + __popc(m & ((1u << lane) - 1u));
         if (in) {
           flag(o, LG_BIASED);
           if (at < LG_BIASES) b_id[at] = int(o), b_val[at] = p.bias_vals[h];
         }
         kept += __popc(m);
       }
-      if (t == 0) s_biases = kept;
+      if (lane == 0) s_biases = kept;
     }
     __syncthreads();
   }
-  const uint32_t* allow = MASK ? p.allowed + int64_t(row) * p.allowed_stride : nullptr;
-  const auto allowed = [&](int o) { return !MASK || ((allow[(c0 + o) >> 5] >> ((c0 + o) & 31)) & 1u); };
+  const auto allowed = [&](int o) { return !MASK || ((s_allow[o >> 5] >> (o & 31)) & 1u); };
   const auto bits = [&](int o) { return TOUCHED ? (cnt[o >> 1] >> (16 * (o & 1))) & 0xffffu : 0u; };
   // token o's value from its logit and bits (the mask apart)
   const auto value = [&](float l, int o, uint32_t c) {
@@ -250,9 +258,9 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
 #pragma unroll
     for (int i = 0; i < LG_EPT; i += 4) {
       if (VEC) {  // four tokens of one mask word and two count words
-        const int at = index(i), g = c0 + at;
+        const int at = index(i);
         uint32_t w = 0xfu;
-        if (MASK) w = at < n ? allow[g >> 5] >> (g & 31) : 0u;
+        if (MASK) w = at < n ? s_allow[at >> 5] >> (at & 31) : 0u;
         uint2 c = make_uint2(0, 0);
         if (TOUCHED) c = *reinterpret_cast<const uint2*>(cnt + (at >> 1));
 #pragma unroll
@@ -309,17 +317,12 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
     }
   }
 
-  // ---- the stream
-  if (n > LG_STEP) load(1, x);
-  for (int step = 1; step < p.steps && step * LG_STEP < n; ++step) {
-    float y[LG_EPT];
-    float top = -INFINITY;
+  // ---- the stream, two steps on their way
+  const int steps = min(p.steps, (n + LG_STEP - 1) / LG_STEP);
+  const auto pass = [&](int step, const float(&y)[LG_EPT]) {
+    float top = y[0];
 #pragma unroll
-    for (int i = 0; i < LG_EPT; ++i) {
-      y[i] = x[i];
-      top = fmaxf(top, y[i]);
-    }
-    if (step + 1 < p.steps && (step + 1) * LG_STEP < n) load(step + 1, x);
+    for (int i = 1; i < LG_EPT; ++i) top = fmaxf(top, y[i]);
     if (top > over) {
 #pragma unroll
       for (int i = 0; i < LG_EPT; ++i) {
@@ -327,7 +330,16 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
         if (y[i] > over && allowed(o) && !(bits(o) & (LG_SEEN | LG_BIASED))) keep(y[i], o);
       }
     }
-    if ((step == 1 || step == 3) && step + 1 < p.steps && (step + 1) * LG_STEP < n) {
+  };
+  float y[LG_EPT];
+  if (steps > 1) load(1, x);
+  if (steps > 2) load(2, y);
+  for (int step = 1; step < steps; step += 2) {
+    pass(step, x);
+    if (step + 2 < steps) load(step + 2, x);
+    if (step + 1 < steps) pass(step + 1, y);
+    if (step + 3 < steps) load(step + 3, y);
+    if (step == 1 && steps > 5) {
       __syncthreads();
       const int have = min(s_n, LG_CAND);
       if (have > p.k) {
@@ -351,7 +363,7 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
   uint64_t* out = p.cand + (int64_t(row) * p.chunks + blockIdx.x) * p.k;
   const int have = s_n;
   if (have <= LG_CAND) {
-    if (have > LG_GROUPS) {  // the same floor once more before the ranking, pair by pair
+    if (have > LG_RANKED) {  // the same floor once more before the ranking, pair by pair
       if (t < LG_GROUPS) {
         uint64_t best = 0;
         for (int i = t; i < have; i += LG_GROUPS) best = max(best, cand[i]);
