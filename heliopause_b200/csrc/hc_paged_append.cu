@@ -20,6 +20,8 @@
 // away.  The first head's row is loaded before the token's sequence is
 // known (rows do not depend on it), and the sequence is found by a 32-way
 // search over the starts, one load per level.
+// Measured: 5044 tokens of 32 / 8 heads of 128 from f32 (186 MB) 41 us, 4.5
+// TB/s, bounded by issue (64%) more than by memory; one token of 64 chats 4.5 us.
 #include "hc_paged.cuh"
 
 namespace hc {

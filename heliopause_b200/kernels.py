@@ -339,7 +339,8 @@ def set_matmul_order(exact: bool) -> None:
 
 
 def device_error() -> None:
-    """Raises CudaKernelError(ERR_TIMEOUT) if a kernel's bounded wait gave up."""
+    """Raises CudaKernelError: ERR_TIMEOUT if a kernel's bounded wait gave up,
+    ERR_SHAPE if a paged batch pointed outside its buffers."""
     assert_cuda_ok(_lib.lib().hpc_device_error(), "deviceStatus")
 
 

@@ -58,7 +58,8 @@ const char *hpc_last_error(void);
 int hpc_version(void);
 
 /* Reads and clears the current device's status word: HPC_ERR_TIMEOUT if a
- * kernel's bounded wait gave up since the last call, else HPC_OK.
+ * kernel's bounded wait gave up since the last call, HPC_ERR_SHAPE if a paged
+ * batch's pages, lengths or starts pointed outside its buffers, else HPC_OK.
  * Synchronizes with the device. */
 int hpc_device_error(void);
 
@@ -278,9 +279,10 @@ int hpc_lm_head_topk_noalloc(hpc_weight lm_head, const float *d_hidden, size_t h
  * query_starts[s + 1] - 1 (its new tokens, in order); kv_lens[s] counts its
  * tokens with the new ones, so row i stands at position kv_lens[s] - new + i;
  * token j is in page page_table[s][j / page_size].  Rows behind
- * query_starts[seqs] belong to no sequence: they are not read and their
- * outputs are left as they were.  A row whose position is negative
- * (kv_lens[s] below its new tokens) is not appended and sees no key.
+ * query_starts[seqs] belong to no sequence: whatever they hold, nothing of
+ * theirs is used, and their outputs are left as they were.  A row whose
+ * position is negative (kv_lens[s] below its new tokens) is not appended and
+ * sees no key.
  * Lengths, starts and tables are read on the device, so captured graphs
  * follow them.  A table entry outside the cache, a length beyond the table or
  * starts outside the rows make the results of that call unspecified, touch
