@@ -799,7 +799,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       for (int s = lane; s < p.b.seqs; s += 32) {
         bool bad;
         const SeqSpan q = seq_span(p.b, s, &bad);
-        const int keys = window > 0 ? min(q.len, window + SPAN / group) : q.len;
+        const int64_t keys = window > 0 ? min(int64_t(q.len), int64_t(window) + SPAN / group) : q.len;
         all_units += int64_t(tiles(q)) * ((keys + PR_KEYS - 1) / PR_KEYS);
       }
 #pragma unroll
@@ -1120,7 +1120,8 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         float mt = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
         // a score of +inf makes the row NaN (inf - inf), as a NaN does
         if (mt == INFINITY) mt = __int_as_float(0x7fffffff);
-        const bool grew = !(mt <= prev) && !((mt - prev) * sc <= PR_GROW);  // prev = -inf and NaN included
+        // prev = -inf and NaN included; rows of no token may hold anything, and are not worth a pass over O
+        const bool grew = lim >= 0 && !(mt <= prev) && !((mt - prev) * sc <= PR_GROW);
         const float now = grew ? mt : prev;
         s_m[lt] = now;
         __syncwarp();

@@ -122,6 +122,34 @@ def test_parts_on_two_streams_and_in_a_graph():
     assert torch.equal(outs[0], want_b) and torch.equal(outs[1], want_c) and torch.equal(outs[2], want_b)
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 200, 1), (128, 257, 1), (256, 96, 1), (64, 1024, 1)])
+@pytest.mark.parametrize("window", [0, 2 ** 31 - 1])
+def test_wide_groups_and_rows_of_no_token(dim, heads, kv_heads, window):
+    # groups around and above a tile's 128 rows, a window wider than any length, and
+    # query rows behind the last sequence that hold NaN and infinities
+    b = ref.Batch([3, 2, 0, 5], [3, 1500, 7, 70], kv_heads, dim, 32, torch.bfloat16, spare_rows=9)
+    q = _q(b, heads, dim, torch.bfloat16)
+    q[b.starts[-1]:] = torch.tensor([torch.nan, torch.inf, -torch.inf] * 3, device="cuda").view(9, 1, 1)
+    out = torch.full((b.rows, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    _, lse = hk.paged_attention(q, b.key, b.value, b.table, b.query_starts, b.kv_lens, max_query_len=5,
+                                scale=dim ** -0.5, window=window, out=out, return_lse=True)
+    assert (out[b.starts[-1]:] == 7.0).all() and (lse[b.starts[-1]:] == -torch.inf).all()
+    n = b.starts[-1]
+    c = b.query_starts.clone()
+    _check(out[:n], lse[:n], b, q[:n], dim ** -0.5, 0)
+    assert torch.equal(c, b.query_starts)
+
+
+@pytest.mark.parametrize("hint", [1, 3, 40, 10 ** 6])
+def test_any_most_new_tokens_gives_the_same_rows(hint):
+    # max_query_len chooses the kernel, not the result
+    b = ref.Batch([40, 1, 7], [2100, 900, 7], 2, 128, 16, torch.float16)
+    q = _q(b, 8, 128, torch.float16)
+    got, lse = hk.paged_attention(q, b.key, b.value, b.table, b.query_starts, b.kv_lens, max_query_len=hint,
+                                  scale=0.08, return_lse=True)
+    _check(got, lse, b, q, 0.08, 0)
+
+
 @pytest.mark.parametrize("dim,heads,kv_heads,dtype", [(256, 8, 2, torch.float16), (64, 6, 3, torch.bfloat16)])
 def test_a_batch_of_chats(dim, heads, kv_heads, dtype):
     """Prompts, decode steps and a verify step of four chats through a cache,
