@@ -1,4 +1,5 @@
-"""Builds libheliocuda.so in-tree with nvcc for sm_100a (no GPU needed).
+"""Builds libheliocuda.so in-tree with nvcc for sm_100a (no GPU needed), and
+the host module _host.so beside it with g++ (csrc/hc_host.cpp, on torch's headers).
 
     python -m heliopause_b200.build          # incremental
     python -m heliopause_b200.build --force  # rebuild everything
@@ -6,9 +7,12 @@
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -16,7 +20,10 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libheliocuda.so"
+HOST_SRC = CSRC / "hc_host.cpp"
+HOST_LIB = PKG / "_host.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CXX = os.environ.get("CXX", "g++")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
@@ -28,6 +35,21 @@ def _sources() -> list[Path]:
 
 def _headers() -> list[Path]:
     return sorted(CSRC.glob("*.cuh")) + sorted((PKG.parent / "include").glob("*.h"))
+
+
+def _build_host(force: bool) -> None:
+    hdr = PKG.parent / "include" / "heliocuda.h"
+    if not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime > max(HOST_SRC.stat().st_mtime, hdr.stat().st_mtime):
+        return
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    inc = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+           Path(shutil.which(NVCC) or NVCC).resolve().parents[1] / "include", hdr.parent]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in inc), str(HOST_SRC), "-o", str(HOST_LIB),
+           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"{CXX} failed on {HOST_SRC.name}")
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
@@ -58,6 +80,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    _build_host(force)
     return LIB
 
 

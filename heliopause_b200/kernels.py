@@ -346,6 +346,25 @@ def device_error() -> None:
 
 # ---- serving many sequences: paged KV cache and its attention ---------------------
 
+# csrc/hc_host.cpp: the four calls below in their plain case, at a third of
+# the host time.  Its functions answer NotImplemented for everything else, which
+# then goes the whole way here.
+_host = None
+
+
+def _load_host():
+    global _host
+    try:
+        from . import _host as module
+    except ImportError as e:
+        raise _lib.LibraryMissing(f"heliopause_b200._host does not load ({e}); run `python -m heliopause_b200.build`") from e
+    lib = _lib.lib()
+    module.bind(*(C.cast(getattr(lib, "hpc_" + name), C.c_void_p).value for name in (
+        "paged_kv_append", "attention_workspace_bytes", "paged_attention", "prompt_attention",
+        "logits_topk_workspace_bytes", "logits_topk")))
+    _host = module
+    return module
+
 _DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -405,6 +424,10 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, v
     [head_dim].  Sequence s owns rows query_starts[s] .. query_starts[s+1];
     kv_lens[s] is its length with them; its token j lies in page
     page_table[s][j // page_size].  Rows behind the last sequence are left."""
+    done = (_host or _load_host()).append(k, v, key_cache, value_cache, page_table, query_starts, kv_lens, q, inv_freq,
+                                          q_norm, k_norm, norm_v, eps, q_out)
+    if done is not NotImplemented:
+        return done
     name = "pagedKvAppend"
     _check_cache(name, key_cache, value_cache)
     dev, dt = key_cache.get_device(), key_cache.dtype
@@ -502,6 +525,11 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     many keys, itself included.  max_query_len: the most rows of a sequence.
     Returns [rows][heads][head_dim] (and the log-sum-exp [rows][heads] with
     return_lse)."""
+    if not return_lse:
+        done = (_host or _load_host()).paged(q, key_cache, value_cache, page_table, query_starts, kv_lens, max_query_len,
+                                             scale, window, out, out_dtype)
+        if done is not NotImplemented:
+            return done
     name = "pagedAttention"
     _check_cache(name, key_cache, value_cache)
     dev, dt = key_cache.get_device(), key_cache.dtype
@@ -539,6 +567,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_st
     (hpc_prompt_attention): q [rows][heads][head_dim], k and v
     [rows][kv_heads][head_dim] (f16 or bf16; views with a row stride allowed),
     sequence s = rows query_starts[s] .. query_starts[s+1]."""
+    if not return_lse:
+        done = (_host or _load_host()).prompt(q, k, v, query_starts, max_query_len, scale, window, out, out_dtype)
+        if done is not NotImplemented:
+            return done
     name = "promptAttention"
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or not q.is_cuda:
         raise CudaKernelError(ERR_SHAPE, f"{name}: q, k and v are [rows][heads][head_dim] device tensors")
@@ -598,6 +630,10 @@ def logits_topk(logits: torch.Tensor, k: int, *, history: torch.Tensor | None = 
     the same for biases with bias_starts; allowed: int32 words of 32 tokens,
     [rows][>= ceil(vocab / 32)].  Logits and their history entries stay as
     they are."""
+    done = (_host or _load_host()).logits(logits, k, history, history_starts, prompt_lens, repetition, frequency, presence,
+                                          bias_ids, bias_values, bias_starts, allowed)
+    if done is not NotImplemented:
+        return done
     name = "logitsTopK"
     if logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda:
         raise CudaKernelError(ERR_TYPE, f"{name}: logits are [rows][vocab] float32 on a device")

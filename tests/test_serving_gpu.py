@@ -229,3 +229,67 @@ def test_a_batch_of_chats(dim, heads, kv_heads, dtype):
                                  token_out=token)
             hist[s].append(int(token))
             assert hist[s][-1] in ids[s].tolist() and (step < 3 or hist[s][-1] == int(ids[s, 0]))
+
+
+class _NothingPlain:
+    """Stands in for the host module: every call goes the whole way in Python."""
+
+    def __getattr__(self, name):
+        return lambda *a: NotImplemented
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_both_host_paths_make_the_same_calls(monkeypatch, dtype):
+    b = ref.Batch([40, 1, 0, 7], [340, 9, 3, 7], 2, 128, 16, dtype, spare_rows=2)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=gen)  # noqa: E731
+    inv = torch.rand(32, device="cuda", dtype=torch.float64, generator=gen)
+    norm = torch.rand(128, device="cuda", generator=gen)
+    x = rnd(b.rows, 12, 128)
+    logits = rnd(3, 7001)
+    i32 = lambda y: torch.tensor(y, dtype=torch.int32, device="cuda")  # noqa: E731
+    f32 = lambda y: torch.tensor(y, dtype=torch.float32, device="cuda")  # noqa: E731
+    full = dict(history=i32([5, 6, 6, 9]), history_starts=i32([0, 3, 3, 4]), prompt_lens=i32([1, 0, 0]),
+                repetition=f32([1.5, 1, 2]), frequency=f32([0.5, 0, 0]), presence=f32([0.1, 0, 0]),
+                bias_ids=i32([7, 8]), bias_values=f32([3.0, -2.0]), bias_starts=i32([0, 1, 1, 2]),
+                allowed=torch.randint(-2 ** 31, 2 ** 31 - 1, (3, 220), dtype=torch.int32, device="cuda", generator=gen))
+
+    def run():
+        key, value = b.key.clone(), b.value.clone()
+        res = []
+        for q, kn, freq in ((x[:, :8], norm, inv), (None, None, None), (x[:, :8], None, inv)):
+            out = torch.zeros((b.rows, 8, 128), dtype=dtype, device="cuda") if q is not None else None
+            r = hk.paged_kv_append(x[:, 8:10], x[:, 10:], key, value, b.table, b.query_starts, b.kv_lens, q=q, inv_freq=freq,
+                                   q_norm=kn, k_norm=kn, norm_v=q is not None, q_out=out)
+            assert r is out
+            res += [key.clone(), value.clone()] + ([r] if r is not None else [])
+        q = x[:, :8].to(dtype)
+        n = b.starts[-1]
+        for kw in ({}, {"window": 5}, {"out_dtype": torch.float32}, {"out": torch.empty_like(q)}):
+            got = hk.paged_attention(q, key, value, b.table, b.query_starts, b.kv_lens, max_query_len=40, scale=0.1, **kw)
+            assert got is kw.get("out", got)
+            res.append(got[:n].clone())
+            k, v = x[:, 8:10].to(dtype), x[:, 10:].to(dtype)
+            got = hk.prompt_attention(q, k, v, b.query_starts, max_query_len=40, scale=1, **kw)
+            assert got is kw.get("out", got)
+            res.append(got[:n].clone())
+        for kw in ({}, full, {"allowed": full["allowed"]}):
+            res += hk.logits_topk(logits, 17, **kw)
+        res += hk.logits_topk(logits[:, 1:6001], 64)
+        with pytest.raises(hk.CudaKernelError):
+            hk.logits_topk(logits, 65)
+        with pytest.raises(hk.CudaKernelError):
+            hk.paged_attention(q, key, value, b.table.long(), b.query_starts, b.kv_lens, max_query_len=40, scale=0.1)
+        with pytest.raises(hk.CudaKernelError):
+            hk.prompt_attention(q, k, v[:1], b.query_starts, max_query_len=40, scale=0.1)
+        with pytest.raises(hk.CudaKernelError):
+            hk.paged_kv_append(x[:, 8:10], x[:, 10:], key, value, b.table, b.query_starts, b.kv_lens, k_norm=norm[:64])
+        return res
+
+    torch.manual_seed(0)
+    fast = run()
+    monkeypatch.setattr(hk, "_host", _NothingPlain())
+    whole = run()
+    assert len(fast) == len(whole)
+    for a, c in zip(fast, whole):
+        assert a.dtype == c.dtype and torch.equal(torch.nan_to_num(a.float(), 9.0), torch.nan_to_num(c.float(), 9.0))
