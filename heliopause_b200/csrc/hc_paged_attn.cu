@@ -73,9 +73,9 @@ struct RowsCfg {
 
 // What the join kernel needs of an item cut by a CTA boundary.
 struct JoinRec {
-  int seq, head, block;  // block < 0: nothing to join
-  int last;              // last CTA that holds tiles of it
-  long long total;       // tiles of the launch
+  int head, block;  // block < 0: nothing to join
+  int row0, n;      // the sequence's rows
+  int last;         // last CTA that may hold tiles of it
 };
 
 struct RowsWork {
@@ -231,7 +231,10 @@ __global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, R
     total += s_sum[i];
   }
   const long long u0 = cta_begin(total, cta, grid), u1 = cta_begin(total, cta + 1, grid);
-  if (u0 >= u1) return;
+  if (u0 >= u1) {  // (fewer tiles than CTAs: the join reads an empty part here)
+    if (t < R) p.w.ml[2 * cta * R + t] = make_float2(-INFINITY, 0.0f);
+    return;
+  }
   if (incl - mine <= u0 && u0 < incl) {
     long long at = incl - mine;
     for (int s = t * per;; ++s) {
@@ -644,10 +647,9 @@ __global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, R
         if (t == 0 && !whole && tile0 == 0) {
           // this CTA holds the item's first tile: it records the join
           JoinRec r;
-          r.seq = w.s, r.head = w.head, r.block = w.block;
+          r.head = w.head, r.block = w.block, r.row0 = q.row0, r.n = q.n;
           const long long last_tile = w.u - w.tile + st.count - 1;
           r.last = int(((last_tile + 1) * grid - 1) / total);
-          r.total = total;
           p.w.rec[cta] = r;
         }
         group_sync();
@@ -662,44 +664,30 @@ __global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, R
 // Joins the partials of the item whose first tile CTA blockIdx.x held, one
 // row per block: the maximum of all, then the sums, by groups of D / 4 threads
 // that take every GROUPS-th partial each (one long sequence leaves a partial on
-// every SM), added up in the groups' order.
+// every SM), added up in the groups' order.  What it waits for is a chain of
+// loads: the record, the maxima, the sums; a CTA that held no tile left an empty
+// partial, so nothing else has to be known.
 constexpr int AJ_THREADS = 256, AJ_PARTS = 512;
 template <class T, int D, int R>
-__global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_constant__ RowsArgs p, int grid) {
+__global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_constant__ RowsArgs p) {
   constexpr int LANES = D / 4, GROUPS = AJ_THREADS / LANES;
-  __shared__ int s_part[AJ_PARTS];
   __shared__ float2 s_ml[AJ_PARTS];
-  __shared__ int s_n;
   __shared__ float s_max[AJ_THREADS / 32];
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ float s_sum[GROUPS];
-  const int c0 = int(blockIdx.x), t = int(threadIdx.x);
+  const int c0 = int(blockIdx.x), r = int(blockIdx.y), t = int(threadIdx.x);
+  const int group = p.a.heads / p.a.kv_heads;
   pdl_wait_prior();
   const JoinRec rec = p.w.rec[c0];
   if (rec.block < 0) return;
-  bool bad;
-  const SeqSpan q = seq_span(p.b, rec.seq, &bad);
-  const int group = p.a.heads / p.a.kv_heads;
   const int r0 = rec.block * R;
-  const int r = int(blockIdx.y);
-  if (r >= min(R, q.n * group - r0)) return;
-  // the partials, in CTA order; a CTA that held no tile left none
-  if (t < 32) {
-    int n = 0;
-    for (int b = c0; b <= rec.last; b += 32) {
-      const int c = b + t;
-      const bool has = c <= rec.last && cta_begin(rec.total, c, grid) < cta_begin(rec.total, c + 1, grid);
-      const unsigned m = __ballot_sync(0xffffffffu, has);
-      if (has) s_part[n + __popc(m & ((1u << t) - 1u))] = c == c0 ? 2 * c + 1 : 2 * c;
-      n += __popc(m);
-    }
-    if (t == 0) s_n = n;
-  }
-  __syncthreads();
-  const int n = s_n;
+  if (r >= min(R, rec.n * group - r0)) return;
+  const int n = rec.last - c0 + 1;
+  // the first CTA's part is its last item, the others' their first
+  const auto slot = [&](int i) { return int64_t(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * R + r; };
   float mx = -INFINITY;
   for (int i = t; i < n; i += AJ_THREADS) {
-    const float2 v = p.w.ml[s_part[i] * R + r];
+    const float2 v = p.w.ml[slot(i)];
     s_ml[i] = v;
     mx = fmaxf(mx, v.x);
   }
@@ -713,11 +701,16 @@ __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_c
   const int g = t / LANES, d = t % LANES * 4;
   float sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
   for (int i = g; i < n; i += GROUPS) {
-    const float f = ex2(s_ml[i].x - ms);
-    const float4 v = *reinterpret_cast<const float4*>(p.w.o + (int64_t(s_part[i]) * R + r) * D + d);
-    sum += f * s_ml[i].y;
+    const float2 s = s_ml[i];
+    // nothing seen there: perhaps nothing was written (and no branch, which would
+    // put the loads behind one another)
+    const bool has = s.x != -INFINITY;
+    const float f = ex2(s.x - ms);
+    float4 v = *reinterpret_cast<const float4*>(p.w.o + slot(has ? i : 0) * D + d);
+    v.x = has ? v.x : 0.0f, v.y = has ? v.y : 0.0f, v.z = has ? v.z : 0.0f, v.w = has ? v.w : 0.0f;
+    sum += f * s.y;
     o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
   }
   s_o[g][t % LANES] = o;
@@ -733,7 +726,7 @@ __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_c
     o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-  const int64_t row = int64_t(q.row0 + (r0 + r) / group) * p.a.heads + rec.head * group + (r0 + r) % group;
+  const int64_t row = int64_t(rec.row0 + (r0 + r) / group) * p.a.heads + rec.head * group + (r0 + r) % group;
   if (p.a.out_f32)
     *reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + row * D + d) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -782,7 +775,7 @@ cudaError_t launch_rows(RowsArgs& p, const KvSource& kv, void* workspace, cudaSt
   e = launch_pdl(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, st, km, vm, p);
   if (e != cudaSuccess) return e;
   static_assert(3 * kMaxSms <= AJ_PARTS, "one partial per CTA at most");
-  return launch_pdl(hc_attn_join_kernel<T, D, Cfg::kRows>, dim3(grid, Cfg::kRows), dim3(AJ_THREADS), 0, st, p, grid);
+  return launch_pdl(hc_attn_join_kernel<T, D, Cfg::kRows>, dim3(grid, Cfg::kRows), dim3(AJ_THREADS), 0, st, p);
 }
 
 template <class T, int D>
