@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(LG_JOIN_THREADS) hc_logits_join_kernel(const _
   uint64_t* cand = keys + n;  // at most k groups of 2 per keys reach the floor
   const uint64_t* in = p.cand + int64_t(row) * n;
   if (t == 0) s_floor = 1, s_n = 0;
+  pdl_launch_next();
   pdl_wait_prior();
 #pragma unroll 8
   for (int i = t; i < n; i += LG_JOIN_THREADS) keys[i] = in[i];

@@ -677,6 +677,7 @@ __global__ void __launch_bounds__(AJ_THREADS) hc_attn_join_kernel(const __grid_c
   __shared__ float s_sum[GROUPS];
   const int c0 = int(blockIdx.x), r = int(blockIdx.y), t = int(threadIdx.x);
   const int group = p.a.heads / p.a.kv_heads;
+  pdl_launch_next();
   pdl_wait_prior();
   const JoinRec rec = p.w.rec[c0];
   if (rec.block < 0) return;

@@ -527,6 +527,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   sync_all<CG>();
   tc_after();
   const uint32_t tmem = s_tmem;
+  pdl_launch_next();  // the next launch sets itself up on the SMs that this one leaves free
   pdl_wait_prior();
   const float sc = fmaxf(fabsf(p.a.scale_log2), 1.2e-38f);
   bool ok = true;
@@ -1258,6 +1259,7 @@ constexpr int PJ_THREADS = 256;
 template <class T, int D>
 __global__ void __launch_bounds__(PJ_THREADS) hc_prompt_join_kernel(const __grid_constant__ PrArgs p) {
   constexpr int SPAN = PR_ROWS * PrCfg<D>::CG, COLS = 32;
+  pdl_launch_next();
   pdl_wait_prior();
   const int lane = int(threadIdx.x) & 31, unit = int(blockIdx.y) * (PJ_THREADS / 32) + (int(threadIdx.x) >> 5);
   const PrJoin it = p.join[blockIdx.x];
