@@ -32,9 +32,9 @@
 // order does not matter).  Chunks are as long as leaves every SM two CTAs, up to
 // 32768 tokens: what a CTA does before and behind the stream, chains of
 // dependent steps of some microseconds, is then paid once.
-// Measured: 64 x 262144 with histories, biases and a mask 46.7 us (69 MB, 1.5
+// Measured: 64 x 262144 with histories, biases and a mask 44.5 us (69 MB, 1.6
 // TB/s; a chunk takes 19 us of such steps and 512 chunks are two rounds of the
-// machine), one row of 262144 11 us, of which the join is 7.7.
+// machine), one row of 262144 9.9 us, two such chains one behind the other.
 #include <algorithm>
 #include <atomic>
 
@@ -55,7 +55,8 @@ constexpr int LG_CAND = 2560;                  // kept keys
 constexpr int LG_FLAGS = 4096;                 // listed tokens with a history or a bias
 // a token's 16 bits: seen in the history, has a bias, times in the output
 constexpr uint32_t LG_SEEN = 0x8000u, LG_BIASED = 0x4000u, LG_COUNT = 0x3fffu;
-constexpr int LG_JOIN_THREADS = 256;
+constexpr int LG_JOIN_THREADS = 1024;
+constexpr int LG_JOIN_GROUP = LG_JOIN_THREADS / LG_GROUPS;  // threads of a group
 constexpr int LG_LISTS = 128;                  // most chunks of a row
 
 struct LogitsArgs {
@@ -422,7 +423,8 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
 // One row's chunk lists -> its ids and values, in the same way: the keys wait in
 // shared memory.  A chunk's list falls with the rank, so a group takes
 // other ranks of every list: of 64 lists of 64 some 90 keys are then above the
-// floor, and one row's join takes 8 us (13.4 with runs of the lists as groups).
+// floor (one row of 262144 takes 9.9 us so, 16.8 with runs of the lists as
+// groups and a quarter of the threads).
 __global__ void __launch_bounds__(LG_JOIN_THREADS) hc_logits_join_kernel(const __grid_constant__ LogitsArgs p) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) uint64_t s_max[LG_GROUPS];
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(LG_JOIN_THREADS) hc_logits_join_kernel(const _
   const int t = int(threadIdx.x), row = int(blockIdx.x);
   const int n = p.chunks * p.k, per = (n + LG_JOIN_THREADS - 1) / LG_JOIN_THREADS;
   uint64_t* keys = reinterpret_cast<uint64_t*>(smem);
-  uint64_t* cand = keys + n;  // at most k groups of 2 per keys reach the floor
+  uint64_t* cand = keys + n;  // at most the keys of k groups reach the floor
   const uint64_t* in = p.cand + int64_t(row) * n;
   if (t == 0) s_floor = 1, s_n = 0;
   pdl_launch_next();
@@ -441,11 +443,13 @@ __global__ void __launch_bounds__(LG_JOIN_THREADS) hc_logits_join_kernel(const _
   __syncthreads();
   uint64_t mx = 0;
   for (int i = 0; i < per; ++i) {
-    const int at = i * LG_JOIN_THREADS + ((t + 37 * i) & (LG_JOIN_THREADS - 1));
+    const int at = i * LG_JOIN_THREADS + ((33 * t + 37 * i) & (LG_JOIN_THREADS - 1));
     if (at < n) mx = max(mx, keys[at]);
   }
-  mx = max(mx, uint64_t(__shfl_xor_sync(0xffffffffu, (unsigned long long)mx, 1)));
-  if ((t & 1) == 0) s_max[t >> 1] = mx;
+#pragma unroll
+  for (int d = 1; d < LG_JOIN_GROUP; d <<= 1)
+    mx = max(mx, uint64_t(__shfl_xor_sync(0xffffffffu, (unsigned long long)mx, d)));
+  if (t % LG_JOIN_GROUP == 0) s_max[t / LG_JOIN_GROUP] = mx;
   __syncthreads();
   if (t < LG_GROUPS) group_floor(s_max, p.k, &s_floor);
   __syncthreads();
@@ -539,7 +543,7 @@ int hpc_logits_topk(const float *d_logits, size_t row_stride, size_t rows, size_
   p.ids = d_ids, p.vals = d_vals;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int per = (p.chunks * p.k + hc::LG_JOIN_THREADS - 1) / hc::LG_JOIN_THREADS;
-  const size_t join = (size_t(p.chunks) * p.k + size_t(2) * p.k * per) * 8;
+  const size_t join = (size_t(p.chunks) * p.k + size_t(hc::LG_JOIN_GROUP) * p.k * per) * 8;
   const size_t cand = size_t(hc::LG_CAND) * 8;
   const size_t smem = cand + (d_history || d_bias_ids ? size_t(p.steps) * hc::LG_STEP * 2 : 0);
   static std::atomic<uint64_t> attr{0};

@@ -38,7 +38,7 @@
 // 402 us with the join, 6.8 TB/s -- a little above a plain copy's rate; 64 chats
 // of 1 to 4096 keys, 8 / 2 heads of 256 (268 MB) 55 us, 4.9 TB/s: there each CTA
 // has 29 tiles and pays some 12 us of starts, page look-ups, merge and join
-// beside them, which is what one chat's token takes (11.5 us).
+// beside them, which is what one chat's token takes (10.8 us).
 #include <algorithm>
 #include <atomic>
 
