@@ -140,6 +140,19 @@ def test_wide_groups_and_rows_of_no_token(dim, heads, kv_heads, window):
     assert torch.equal(c, b.query_starts)
 
 
+@pytest.mark.parametrize("dim,heads", [(256, 12), (128, 8), (64, 4)])
+def test_many_sequences_in_parts(dim, heads):
+    # more sequences than one look at their lengths takes in, some of them empty,
+    # and few enough items that the long ones are cut into parts
+    new = [20 + i % 3 if i % 5 else 0 for i in range(43)]
+    lens = [max(n, (i * 977) % 2900) for i, n in enumerate(new)]
+    b = ref.Batch(new, lens, 1, dim, 16, torch.bfloat16, spare_rows=1)
+    q = _q(b, heads, dim, torch.bfloat16)
+    got, lse = hk.paged_attention(q, b.key, b.value, b.table, b.query_starts, b.kv_lens, max_query_len=max(new),
+                                  scale=dim ** -0.5, return_lse=True)
+    _check(got, lse, b, q, dim ** -0.5, 0)
+
+
 @pytest.mark.parametrize("hint", [1, 3, 40, 10 ** 6])
 def test_any_most_new_tokens_gives_the_same_rows(hint):
     # max_query_len chooses the kernel, not the result
