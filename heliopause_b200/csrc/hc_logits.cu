@@ -346,6 +346,9 @@ __global__ void __launch_bounds__(LG_THREADS, 2) hc_logits_chunk_kernel(const __
     if (step == 1 && steps > 5) {
       __syncthreads();
       const int have = min(s_n, LG_CAND);
+      // all warps have read s_n before one of them keeps a key again: the
+      // barriers below stand behind what was read
+      __syncthreads();
       if (have > p.k) {
         if (t < LG_GROUPS) {
           uint64_t best = 0;
