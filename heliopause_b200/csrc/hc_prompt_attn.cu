@@ -49,8 +49,8 @@
 // swizzled, which is the operand layout of both products (K rows are K-major; V is
 // N-major as it lies).  Keys that a row does not see get -inf scores and add
 // nothing: values behind the last key in use are zeroed before they are
-// multiplied, and if a value that only some rows of a tile see is not finite
-// (0 * inf), the tile's rows are summed again by plain loops over what they see.
+// multiplied, and so is a value that only some rows of a tile see and that is not
+// finite (0 * inf); it is added to the stored rows that see it afterwards.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -93,9 +93,8 @@ static_assert(2 * PR_REGS_SOFTMAX + 2 * PR_REGS_OTHER == 4 * 128, "the split is 
 struct PrArgs {
   AttnArgs a;
   PagedBatch b;
-  const void* k;       // for the plain loops
-  const void* v;
-  int64_t k_stride, v_stride;
+  const void* v;       // read again where a value is not finite
+  int64_t v_stride;
   int box_k, box_v;    // key rows per TMA copy, as powers of two
   int whole_k, whole_v;  // a copy brings the CTA's whole tile, every piece of it
   int64_t slots;
@@ -351,68 +350,23 @@ __device__ __forceinline__ void pr_tma_q(uint32_t dst, const CUtensorMap* map, i
 }
 constexpr uint32_t kLeaderMask = 0xfeffffffu;  // a shared::cluster address in the pair's even CTA
 
-// ---- the tile's sums by plain loops -----------------------------------------------
-
-// One row of a tile, from global memory: keys [lo, hi] of sequence `s`.  Only
-// for tiles where a value that some rows do not see is not finite.
-template <class T, int D>
-__device__ __forceinline__ void pr_plain_row(const PrArgs& p, int s, int row0, int kv_head, const T* q, int lo, int hi,
-                                          T* out, float* out32, float* lse, float2* part) {
-  const auto at = [&](const void* base, int64_t stride, int j) {
-    int64_t r = row0 + int64_t(j);
-    if (p.b.table) {
-      const int page = p.b.table[int64_t(s) * p.b.width + (j >> p.b.page_shift)];
-      const bool in = page >= 0 && page < p.b.pages;
-      r = ((in ? int64_t(page) : 0) << p.b.page_shift) + (j & ((1 << p.b.page_shift) - 1));
-    }
-    return static_cast<const T*>(base) + r * stride + int64_t(kv_head) * D;
-  };
-  const auto score = [&](int j) {
-    const T* k = at(p.k, p.k_stride, j);
-    float d = 0.0f;
-#pragma unroll 1
-    for (int i = 0; i < D; i += 2) {
-      const float2 x = HalfOps<T>::unpack(*reinterpret_cast<const uint32_t*>(q + i));
-      const float2 y = HalfOps<T>::unpack(*reinterpret_cast<const uint32_t*>(k + i));
-      d = fmaf(x.x, y.x, d);
-      d = fmaf(x.y, y.y, d);
-    }
-    return d * p.a.scale_log2;
-  };
-  float m = -INFINITY;
-#pragma unroll 1
-  for (int j = lo; j <= hi; ++j) m = fmaxf(m, score(j));
-  const float ms = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-  for (int c = 0; c < D; c += 4) {
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 1
-    for (int j = lo; j <= hi; ++j) {
-      const float e = ex2(score(j) - ms);
-      const uint2 v = *reinterpret_cast<const uint2*>(at(p.v, p.v_stride, j) + c);
-      const float2 a = HalfOps<T>::unpack(v.x), b = HalfOps<T>::unpack(v.y);
-      l += e;
-      o.x = fmaf(e, a.x, o.x), o.y = fmaf(e, a.y, o.y), o.z = fmaf(e, b.x, o.z), o.w = fmaf(e, b.y, o.w);
-    }
-    if (part) {  // as a part's other rows lie
-      *reinterpret_cast<float4*>(out32 + c * 32) = o;
-      if (c == 0) *part = make_float2(m, l);
-      continue;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    if (out32) *reinterpret_cast<float4*>(out32 + c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    else
-      *reinterpret_cast<uint2*>(out + c) =
-          make_uint2(HalfOps<T>::pack(o.x * inv, o.y * inv), HalfOps<T>::pack(o.z * inv, o.w * inv));
-    if (c == 0 && lse) *lse = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
-  }
-}
+// ---- values that are not finite
 
 template <class T>
 __device__ __forceinline__ bool pr_not_finite(uint32_t v) {
   constexpr uint32_t e = sizeof(T) && HalfOps<T>::kMap == CU_TENSOR_MAP_DATA_TYPE_FLOAT16 ? 0x7c00u : 0x7f80u;
   return (v & e) == e || ((v >> 16) & e) == e;
+}
+// The two values of a word, 0 in the place of those that are not finite.
+template <class T>
+__device__ __forceinline__ uint32_t pr_finite(uint32_t v) {
+  return (pr_not_finite<T>(v & 0xffffu) ? 0u : v & 0xffffu) | (pr_not_finite<T>(v >> 16) ? 0u : v & 0xffff0000u);
+}
+// x + v where v is not finite, else x.
+template <class T>
+__device__ __forceinline__ float2 pr_add_odd(float2 x, uint32_t v) {
+  const float2 f = HalfOps<T>::unpack(v);
+  return make_float2(pr_not_finite<T>(v & 0xffffu) ? x.x + f.x : x.x, pr_not_finite<T>(v >> 16) ? x.y + f.y : x.y);
 }
 
 // ---- the kernel ---------------------------------------------------------------------
@@ -457,6 +411,19 @@ __device__ __forceinline__ PrGeom pr_geom(const PrItem& it, int group, int windo
     g.units = 0;
   }
   return g;
+}
+
+// Keys [all_lo, all_hi] are seen by every row of the item (in a pair each
+// CTA looks after half of every value for both).
+struct PrBorder {
+  int all_lo, all_hi;
+  __device__ __forceinline__ bool tile(int k0) const { return k0 + PR_KEYS - 1 > all_hi || k0 < all_lo; }
+  // of a tile's keys the first that some row may not see
+  __device__ __forceinline__ int seen(int k0) const { return k0 < all_lo ? 0 : max(0, all_hi + 1 - k0); }
+};
+__device__ __forceinline__ PrBorder pr_border(const PrItem& it, const PrGeom& g, int group, int window, int rows_per_item) {
+  return {window > 0 ? g.pos0 + (min(g.r0 + rows_per_item, g.nrows) - 1) / group - window + 1 : 0,
+          min(it.span.len - 1, g.pos0 + g.r0 / group)};
 }
 
 template <class T, int D>
@@ -807,6 +774,58 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       for (int d = 1; d < 32; d <<= 1) all_units += __shfl_xor_sync(0xffffffffu, all_units, d);
     }
     uint32_t nq = 0, v0 = 0, ends = 0;  // items with tiles whose Q was asked for; tiles and items with tiles that ended
+    // The values that the softmax warps took out of an item's border tiles, added
+    // to the warp's stored rows that see them.  A lane takes two values of every
+    // 64, of one key after the other, so no two lanes meet in a row.
+    const auto add_odd = [&](const PrItem& it, const PrGeom& g, int tok0, int rem, bool live) {
+      const PrBorder border = pr_border(it, g, group, window, SPAN);
+      const int pos = g.pos0 + row_at(tok0, rem, live ? w4 * 32 + lane : 0).x;
+      const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
+#pragma unroll 1
+      for (int u = 0; u < g.units; ++u) {
+        const int k0 = g.key0 + u * PR_KEYS, end = min(k0 + PR_KEYS, g.key_hi);
+        if (!border.tile(k0)) continue;
+#pragma unroll 1
+        for (int j = k0 + border.seen(k0); j < end; ++j) {
+          int64_t row = it.span.row0 + int64_t(j);
+          if (p.b.table) {
+            const int page = p.b.table[int64_t(it.seq) * p.b.width + (j >> p.b.page_shift)];
+            if (page < 0 || page >= p.b.pages) continue;  // (its values were taken as 0)
+            row = (int64_t(page) << p.b.page_shift) + (j & ((1 << p.b.page_shift) - 1));
+          }
+          const T* const src = static_cast<const T*>(p.v) + row * p.v_stride + int64_t(it.head) * D + lane * 2;
+          uint32_t v[D / 64];
+          bool here = false;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            v[c] = *reinterpret_cast<const uint32_t*>(src + c * 64);
+            here = here || pr_not_finite<T>(v[c]);
+          }
+          if (!__any_sync(0xffffffffu, here)) continue;
+          for (unsigned rows = __ballot_sync(0xffffffffu, j <= lim && j >= low); rows; rows &= rows - 1) {
+            const int r = __ffs(rows) - 1;
+            const int2 own = row_at(tok0, rem, w4 * 32 + r);
+            const int64_t at = (int64_t(it.span.row0 + own.x) * p.a.heads + it.head * group + own.y) * D;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              if (!pr_not_finite<T>(v[c])) continue;
+              const int d = c * 64 + lane * 2;
+              if (it.parts > 1 || p.a.out_f32) {
+                float* const to = it.parts > 1 ? p.part_o + (int64_t(it.place) * SPAN + int(rank) * PR_ROWS + w4 * 32) * D +
+                                                     (d >> 2) * 128 + r * 4 + (d & 2)
+                                               : static_cast<float*>(p.a.out) + at + d;
+                *reinterpret_cast<float2*>(to) = pr_add_odd<T>(*reinterpret_cast<const float2*>(to), v[c]);
+              } else {
+                uint32_t* const to = reinterpret_cast<uint32_t*>(static_cast<T*>(p.a.out) + at + d);
+                const float2 x = pr_add_odd<T>(HalfOps<T>::unpack(*to), v[c]);
+                *to = HalfOps<T>::pack(x.x, x.y);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+    };
     // An item's rows, once its last product has landed: a lane has a row's sums.
     const auto put_rows = [&](const PrItem& it, int n) {
       const PrGeom g = pr_geom(it, group, window, SPAN);
@@ -841,19 +860,18 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         // a part leaves its sums undivided: [warp's 32 rows][head_dim / 4][row] float4
         const int64_t rows = int64_t(it.place) * SPAN + int(rank) * PR_ROWS + w4 * 32;
         float* const to = p.part_o + rows * D + lane * 4;
-        if (!odd) {
-          p.part_ml[rows + lane] = make_float2(m * sc, l);
+        p.part_ml[rows + lane] = make_float2(m * sc, l);
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t o[16];
-            tm_ld16(oa + c, o);
-            tm_wait_ld();
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tm_ld16(oa + c, o);
+          tm_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<uint4*>(to + (c + e) * 32) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<uint4*>(to + (c + e) * 32) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
-      } else if (!odd) {
+        done_with_o();
+      } else {
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
         const int64_t tok = int64_t(it.span.row0 + tok0) * p.a.heads + it.head * group;
         if (live && p.a.lse) {
@@ -922,22 +940,8 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           flush(c * esz);
         }
       }
-      if (it.parts > 1 || odd) done_with_o();
-      if (odd && (live || it.parts > 1)) {
-        const int2 own = row_at(tok0, rem, live ? rr : 0);
-        const int pos = g.pos0 + own.x, lim = live ? min(pos, it.span.len - 1) : -1;
-        const int low = window > 0 ? max(0, pos - window + 1) : 0;
-        const T* q = static_cast<const T*>(p.a.q) + int64_t(it.span.row0 + own.x) * p.a.q_stride + (it.head * group + own.y) * D;
-        const int64_t row = int64_t(it.span.row0 + own.x) * p.a.heads + it.head * group + own.y;
-        const int64_t rows = int64_t(it.place) * SPAN + int(rank) * PR_ROWS + w4 * 32;
-        const bool part = it.parts > 1;
-        pr_plain_row<T, D>(p, it.seq, it.span.row0, it.head, q, part ? max(low, g.key0) : low,
-                           part ? min(lim, g.key_hi - 1) : lim, static_cast<T*>(p.a.out) + row * D,
-                           part ? p.part_o + rows * D + lane * 4
-                                : p.a.out_f32 ? static_cast<float*>(p.a.out) + row * D : nullptr,
-                           p.a.lse ? p.a.lse + row : nullptr, part ? p.part_ml + rows + lane : nullptr);
-      }
       __syncwarp();
+      if (odd) add_odd(it, g, tok0, rem, live);
     };
     int x = int(blockIdx.x) / CG;
     PrItem prev;
@@ -1072,10 +1076,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       const int pos = g.pos0 + own.x;
       const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
       float m = -INFINITY, l = 0.0f;
-      // keys [all_lo, all_hi] are seen by every row of the item (in a pair
-      // each CTA looks after half of every value for both)
-      const int all_hi = min(it.span.len - 1, g.pos0 + g.r0 / group);
-      const int all_lo = window > 0 ? g.pos0 + (min(g.r0 + SPAN, g.nrows) - 1) / group - window + 1 : 0;
+      const PrBorder border = pr_border(it, g, group, window, SPAN);
       for (int u = int((v0 ^ uint32_t(wg)) & 1u); u < g.units; u += 2) {
         const uint32_t v = v0 + uint32_t(u);
         const int k0 = g.key0 + u * PR_KEYS;
@@ -1097,13 +1098,13 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           __syncwarp();
           if (lane == 0 && ok) arrive_leader<CG>(&s_free[wg]);
         }
-        const bool edge = k0 + PR_KEYS - 1 > all_hi || k0 < all_lo;
+        const bool edge = border.tile(k0);
         if (edge) {
           const int hi = lim - k0, lo = low - k0;
 #pragma unroll
           for (int c = 0; c < PR_KEYS; ++c)
             if (c > hi) s[c] = 0xff800000u;
-          if (k0 < all_lo) {
+          if (k0 < border.all_lo) {
 #pragma unroll
             for (int c = 0; c < PR_KEYS; ++c)
               if (c < lo) s[c] = 0xff800000u;
@@ -1174,27 +1175,31 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
           l += a + b;
         }
         if (edge) {
-          // values that only some rows see are looked through for what is not
-          // finite; values behind the last key in use become 0 up to the next
-          // 16 (the product goes no further)
+          // values that only some rows see and that are not finite become 0 for
+          // the product (0 * inf); the item warps add them to the rows that see
+          // them.  Values behind the last key in use become 0 up to the next 16
+          // (the product goes no further).
           constexpr int CH = Cfg::kPiecesV * 8;  // 16-byte chunks of a key's values in this CTA
           const uint32_t st = v % ST, vt = sv + st * Cfg::kK;
-          const int used = min(PR_KEYS, g.key_hi - k0), seen = k0 < all_lo ? 0 : max(0, all_hi + 1 - k0);
+          const int used = min(PR_KEYS, g.key_hi - k0), seen = border.seen(k0);
           const auto chunk = [&](int i) {
             return vt + (i % CH >> 3) * (PR_KEYS * 128) + i / CH * 128 + ((i & 7) << 4);
           };
           ok = ok && pr_wait(&v_full[st], (v / ST) & 1u, err);
           ok = __all_sync(0xffffffffu, ok);
           bool odd = false;
+          const auto load = [&](int i, uint32_t(&w)[4]) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(chunk(i))
+                         : "memory");
+          };
           if (ok) {
 #pragma unroll 4
             for (int i = seen * CH + lt; i < used * CH; i += 128) {
-              uint32_t a, b, d, e;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(a), "=r"(b), "=r"(d), "=r"(e)
-                           : "r"(chunk(i))
-                           : "memory");
-              odd = odd || pr_not_finite<T>(a) || pr_not_finite<T>(b) || pr_not_finite<T>(d) || pr_not_finite<T>(e);
+              uint32_t w[4];
+              load(i, w);
+              odd = odd || pr_not_finite<T>(w[0]) || pr_not_finite<T>(w[1]) || pr_not_finite<T>(w[2]) || pr_not_finite<T>(w[3]);
             }
             if (used & 15) {
               for (int i = used * CH + lt; i < (used + 15 & ~15) * CH; i += 128)
@@ -1202,7 +1207,19 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
           }
-          if (__any_sync(0xffffffffu, odd) && lane == 0) {
+          odd = __any_sync(0xffffffffu, odd);
+          if (odd) {
+#pragma unroll 1
+            for (int i = seen * CH + lt; i < used * CH; i += 128) {
+              uint32_t w[4];
+              load(i, w);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk(i)), "r"(pr_finite<T>(w[0])),
+                           "r"(pr_finite<T>(w[1])), "r"(pr_finite<T>(w[2])), "r"(pr_finite<T>(w[3]))
+                           : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          if (odd && lane == 0) {
             // both CTAs' rows are the sums of both CTAs' dims
             for (int c = 0; c < CG; ++c) {
               if constexpr (CG == 1)
@@ -1216,7 +1233,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
             }
           }
           // what was written here is read by the pair's products, and its flag by the other CTA
-          if (CG == 2 && ((used & 15) || __any_sync(0xffffffffu, odd))) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          if (CG == 2 && (odd || (used & 15))) asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
         tm_wait_st();
         tc_before();
@@ -1394,9 +1411,7 @@ cudaError_t launch_attn_prompt(const AttnArgs& a, const PagedBatch& b, const KvS
   PrArgs p{};
   p.a = a;
   p.b = b;
-  p.k = kv.k;
   p.v = kv.v;
-  p.k_stride = int64_t(kv.k_stride);
   p.v_stride = int64_t(kv.v_stride);
   return kv.dtype == HPC_DTYPE_F16 ? launch_prompt_t<__half>(p, kv, workspace, st)
                                    : launch_prompt_t<__nv_bfloat16>(p, kv, workspace, st);
