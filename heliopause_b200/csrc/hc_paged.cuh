@@ -61,6 +61,14 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedBatch& b, int s, bool* ba
   return q;
 }
 
+// The first key that a row at position `pos` sees (window 0: all of them).  A
+// position is negative where kv_lens is below the new tokens, so it is compared
+// before anything is taken from it: with a window near 2^31 the
+// difference would not fit.
+__device__ __forceinline__ int first_key(int pos, int window) {
+  return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
+
 template <class T>
 struct HalfOps;
 template <>

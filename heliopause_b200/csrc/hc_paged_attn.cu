@@ -134,8 +134,7 @@ struct SeqTiles {
 template <int R>
 __device__ __forceinline__ SeqTiles seq_tiles(const SeqSpan& q, int group, int window) {
   SeqTiles t;
-  const int low = window > 0 ? max(0, q.len - q.n - window + 1) : 0;
-  t.first = low / AR_TILE;
+  t.first = first_key(q.len - q.n, window) / AR_TILE;
   t.count = max(1, (q.len + AR_TILE - 1) / AR_TILE - t.first);
   t.blocks = (q.n * group + R - 1) / R;
   return t;
@@ -154,7 +153,7 @@ __device__ __forceinline__ BlockSpan block_span(const SeqSpan& q, int block, int
   s.rows = min(R, q.n * group - r0);
   s.pos0 = q.len - q.n;  // position of the sequence's first new token
   const int p_first = s.pos0 + r0 / group, p_last = s.pos0 + (r0 + s.rows - 1) / group;
-  s.lo = window > 0 ? max(0, p_first - window + 1) : 0;
+  s.lo = first_key(p_first, window);
   s.hi = min(q.len, p_last + 1);
   return s;
 }
@@ -374,7 +373,7 @@ __global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, R
             const int r = nb * 8 + lc * 2 + e;
             const int pos = sp.pos0 + (r0 + r) / group;
             lim[nb][e] = r < rows ? min(pos, q.len - 1) : -1;
-            low[nb][e] = window > 0 ? pos - window + 1 : 0;
+            low[nb][e] = first_key(pos, window);
             m[nb][e] = -INFINITY;
             l[nb][e] = 0.0f;
           }
@@ -386,7 +385,7 @@ __global__ void __launch_bounds__(RowsCfg<D, NB, RG>::kThreads, RowsCfg<D, NB, R
             for (int e = 0; e < 4; ++e) o[nb][k][e] = 0.0f;
         // every key of [all_lo, all_hi] is seen by every row of the group
         const int all_hi = min(q.len - 1, sp.pos0 + r0 / group);
-        const int all_lo = window > 0 ? sp.pos0 + (r0 + rows - 1) / group - window + 1 : 0;
+        const int all_lo = first_key(sp.pos0 + (r0 + rows - 1) / group, window);
         const int tile0 = w.tile;
         for (; w.tile < st.count && w.u < w.end; ++w.tile, ++w.u) {
           const int k0 = (st.first + w.tile) * AR_TILE;

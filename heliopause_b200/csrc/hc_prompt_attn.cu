@@ -398,7 +398,7 @@ __device__ __forceinline__ PrGeom pr_geom(const PrItem& it, int group, int windo
   g.r0 = it.tile * rows_per_item;
   g.pos0 = it.span.len - it.span.n;
   const int p_first = g.pos0 + g.r0 / group, p_last = g.pos0 + (min(g.r0 + rows_per_item, g.nrows) - 1) / group;
-  const int key_lo = window > 0 ? max(0, p_first - window + 1) : 0;
+  const int key_lo = first_key(p_first, window);
   g.key_hi = min(it.span.len, p_last + 1);
   g.key0 = key_lo / PR_KEYS * PR_KEYS;
   g.units = g.key_hi > key_lo ? (g.key_hi - g.key0 + PR_KEYS - 1) / PR_KEYS : 0;
@@ -422,7 +422,7 @@ struct PrBorder {
   __device__ __forceinline__ int seen(int k0) const { return k0 < all_lo ? 0 : max(0, all_hi + 1 - k0); }
 };
 __device__ __forceinline__ PrBorder pr_border(const PrItem& it, const PrGeom& g, int group, int window, int rows_per_item) {
-  return {window > 0 ? g.pos0 + (min(g.r0 + rows_per_item, g.nrows) - 1) / group - window + 1 : 0,
+  return {first_key(g.pos0 + (min(g.r0 + rows_per_item, g.nrows) - 1) / group, window),
           min(it.span.len - 1, g.pos0 + g.r0 / group)};
 }
 
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     const auto add_odd = [&](const PrItem& it, const PrGeom& g, int tok0, int rem, bool live) {
       const PrBorder border = pr_border(it, g, group, window, SPAN);
       const int pos = g.pos0 + row_at(tok0, rem, live ? w4 * 32 + lane : 0).x;
-      const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
+      const int lim = live ? min(pos, it.span.len - 1) : -1, low = first_key(pos, window);
 #pragma unroll 1
       for (int u = 0; u < g.units; ++u) {
         const int k0 = g.key0 + u * PR_KEYS, end = min(k0 + PR_KEYS, g.key_hi);
@@ -1074,7 +1074,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
       const bool live = rt + lt < g.nrows;
       const int2 own = row_at(tok0, rem, live ? lt : 0);  // token, head of the group
       const int pos = g.pos0 + own.x;
-      const int lim = live ? min(pos, it.span.len - 1) : -1, low = window > 0 ? pos - window + 1 : 0;
+      const int lim = live ? min(pos, it.span.len - 1) : -1, low = first_key(pos, window);
       float m = -INFINITY, l = 0.0f;
       const PrBorder border = pr_border(it, g, group, window, SPAN);
       for (int u = int((v0 ^ uint32_t(wg)) & 1u); u < g.units; u += 2) {
