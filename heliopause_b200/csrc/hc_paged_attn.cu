@@ -867,8 +867,10 @@ int hpc_paged_check(const char* what, size_t heads, size_t kv_heads, size_t head
   if (page_size) {
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
       return hpc_fail(HPC_ERR_SHAPE, "%s: page_size %zu (a power of two from 16 to 1024)", what, page_size);
-    if (pages < 1 || pages > (size_t(INT32_MAX) - 1024) / page_size || table_width < 1 ||
-        table_width > size_t(INT32_MAX) / page_size)
+    // slots and positions are 32-bit numbers, and a tile's end may lie up to 128
+    // behind the last of them
+    const size_t most = (size_t(INT32_MAX) - 1024) / page_size;
+    if (pages < 1 || pages > most || table_width < 1 || table_width > most)
       return hpc_fail(HPC_ERR_SHAPE, "%s: %zu pages, a table of %zu", what, pages, table_width);
   }
   return HPC_OK;

@@ -273,8 +273,9 @@ int hpc_lm_head_topk_noalloc(hpc_weight lm_head, const float *d_hidden, size_t h
  *
  * Cache: keys and values [pages][page_size][kv_heads][head_dim], f16 or
  * bf16; page_size a power of two from 16 to 1024, head_dim 64, 128 or 256,
- * heads a multiple of kv_heads (query head h reads KV head
- * h / (heads / kv_heads)).
+ * heads (at most 1024) a multiple of kv_heads (query head h reads KV head
+ * h / (heads / kv_heads)).  pages * page_size and table_width * page_size are
+ * at most 2^31 - 1025, rows * heads below 2^31, sequences at most 2^20.
  * Batch: sequence s owns the packed rows query_starts[s] ..
  * query_starts[s + 1] - 1 (its new tokens, in order); kv_lens[s] counts its
  * tokens with the new ones, so row i stands at position kv_lens[s] - new + i;
