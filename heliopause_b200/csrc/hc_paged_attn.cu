@@ -918,6 +918,18 @@ int attention(const char* what, const void* d_q, size_t q_stride, const hc::KvSo
   const size_t need = workspace_need(head_dim);
   if (workspace_bytes < need)
     return hpc_fail(HPC_ERR_SHAPE, "%s: a workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  // Rows are written while keys, values and other rows' queries are still read.
+  // Only a row's own query is behind it then, so `out` may be q itself.
+  const auto bytes = [&](uint64_t rows, uint64_t stride, size_t row) { return ((rows - 1) * stride + row) * 2; };
+  const auto meets = [&](const void* p, uint64_t n) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(p), o = reinterpret_cast<uintptr_t>(d_out);
+    return x < o + uint64_t(b.rows) * heads * head_dim * (out_dtype == HPC_DTYPE_F32 ? 4 : 2) && o < x + n;
+  };
+  const bool in_place = d_out == d_q && out_dtype == kv.dtype && q_stride == heads * head_dim;
+  if ((!in_place && meets(d_q, bytes(b.rows, q_stride, heads * head_dim))) ||
+      meets(kv.k, bytes(kv.slots, kv.k_stride, kv_heads * head_dim)) ||
+      meets(kv.v, bytes(kv.slots, kv.v_stride, kv_heads * head_dim)))
+    return hpc_fail(HPC_ERR_ARG, "%s: the output lies over keys, values or other queries", what);
   hc::AttnArgs a{};
   a.q = d_q;
   a.q_stride = int64_t(q_stride);

@@ -523,6 +523,7 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     (hpc_paged_attention): decode (one row each), verify, or chunks of
     prompts.  Arguments as paged_kv_append's; window > 0: a row sees that
     many keys, itself included.  max_query_len: the most rows of a sequence.
+    out may be a contiguous q itself, and lies over no other input.
     Returns [rows][heads][head_dim] (and the log-sum-exp [rows][heads] with
     return_lse)."""
     if not return_lse:

@@ -327,7 +327,8 @@ int hpc_attention_workspace_bytes(size_t heads, size_t kv_heads, size_t head_dim
  * maxima, sums and outputs are f32; probabilities are rounded to the cache's
  * type before they multiply the values.  max_query_len: the most new tokens
  * of any sequence (1 for a decode step); it chooses the kernel, not the
- * result. */
+ * result.  out may be q itself (of q's type, q contiguous); an out that lies over
+ * keys, values or q in any other way is refused. */
 int hpc_paged_attention(const void *d_q, size_t q_stride, const void *d_key_cache, const void *d_value_cache,
                         int cache_dtype, size_t pages, size_t page_size, const int32_t *d_page_table,
                         size_t table_width, const int32_t *d_query_starts, const int32_t *d_kv_lens, size_t seqs,
