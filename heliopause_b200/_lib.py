@@ -6,7 +6,9 @@ calls raise.  The declarations mirror include/heliocuda.h one for one.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.metadata
 import re
+import sys
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -123,6 +125,12 @@ def lib() -> C.CDLL:
             f.argtypes = args
         _lib = L
     return _lib
+
+
+def host_built_for() -> str:
+    """What _host.so is bound to: torch's C++ interface and Python's are not
+    the same from version to version."""
+    return f"torch {importlib.metadata.version('torch')}, python {sys.version_info[0]}.{sys.version_info[1]}"
 
 
 def last_error() -> str:

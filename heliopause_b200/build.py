@@ -16,6 +16,8 @@ import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
+from . import _lib
+
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
@@ -39,17 +41,21 @@ def _headers() -> list[Path]:
 
 def _build_host(force: bool) -> None:
     hdr = PKG.parent / "include" / "heliocuda.h"
-    if not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime > max(HOST_SRC.stat().st_mtime, hdr.stat().st_mtime):
+    stamp = OBJ / "_host.built_for"
+    if not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime > max(HOST_SRC.stat().st_mtime, hdr.stat().st_mtime) \
+            and stamp.exists() and stamp.read_text() == _lib.host_built_for():
         return
     torch = Path(importlib.util.find_spec("torch").origin).parent
     inc = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
            Path(shutil.which(NVCC) or NVCC).resolve().parents[1] / "include", hdr.parent]
-    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in inc), str(HOST_SRC), "-o", str(HOST_LIB),
-           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f'-DHC_BUILT_FOR="{_lib.host_built_for()}"',
+           *(f"-I{i}" for i in inc), str(HOST_SRC), "-o", str(HOST_LIB), f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError(f"{CXX} failed on {HOST_SRC.name}")
+    stamp.write_text(_lib.host_built_for())
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:

@@ -352,4 +352,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  // the versions whose interfaces were compiled in; the caller compares them before its first call
+  if (m && PyModule_AddStringConstant(m, "built_for", HC_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import warnings
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -352,13 +353,30 @@ def device_error() -> None:
 _host = None
 
 
+class _NoHost:
+    """In the host module's place where it does not load: every call goes the
+    whole way here, to the same kernels."""
+
+    @staticmethod
+    def append(*args):
+        return NotImplemented
+
+    paged = prompt = logits = append
+
+
 def _load_host():
     global _host
+    lib = _lib.lib()
     try:
         from . import _host as module
+        built_for = getattr(module, "built_for", "another version")
+        if built_for != _lib.host_built_for():
+            raise ImportError(f"it was built for {built_for}")
     except ImportError as e:
-        raise _lib.LibraryMissing(f"heliopause_b200._host does not load ({e}); run `python -m heliopause_b200.build`") from e
-    lib = _lib.lib()
+        warnings.warn(f"heliopause_b200._host does not load ({e}): serving calls take some 10 us longer on the host; run "
+                      "`python -m heliopause_b200.build`", RuntimeWarning, stacklevel=3)
+        _host = _NoHost
+        return _host
     module.bind(*(C.cast(getattr(lib, "hpc_" + name), C.c_void_p).value for name in (
         "paged_kv_append", "attention_workspace_bytes", "paged_attention", "prompt_attention",
         "logits_topk_workspace_bytes", "logits_topk")))
