@@ -440,6 +440,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
   __shared__ __align__(16) uint4 clc_resp;
   __shared__ __align__(8) uint64_t q_full[2], q_free[2], k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], v_peer[ST];
   __shared__ __align__(8) uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free, m_pass[4], l_pass[4], l_free;
+  __shared__ __align__(8) uint64_t pv_seen[2][4];
   __shared__ __align__(8) uint64_t item_full[2], item_empty[2], clc_full, clc_ready, near_end;
   __shared__ PrItem s_items[2];
   __shared__ uint32_t s_tmem;
@@ -481,6 +482,7 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
     }
     for (int w = 0; w < 4; ++w) {
       mbar_init(&m_pass[w], 1);
+      for (int i = 0; i < 2; ++i) mbar_init(&pv_seen[i][w], 1);
       mbar_init(&l_pass[w], 2);
     }
     mbar_init(&o_free, ITEM_WARPS * CG);
@@ -1134,7 +1136,14 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         }
         if (__any_sync(0xffffffffu, grew) && u > 0) {
           const float f = grew ? ex2((prev - mt) * sc) : 1.0f;
-          // O to the new m, once the product before has landed
+          // O to the new m, once the product before has landed.  A parity tells a
+          // phase from the next only: where values arrive late, the product of tile v - 3
+          // may still be on its way when the scores of tile v are here, and its
+          // barrier then reads as if that of tile v - 1 had landed.  The other
+          // warpgroup waits for the former on its way to tile v - 1's P, so it says when
+          // it has.  (Where P lies in its S slot, the scores of tiles v - 1 and v were issued
+          // and committed behind that product, by the same thread, and have landed.)
+          if constexpr (Cfg::kOwnP) ok = ok && pr_wait(&pv_seen[wg ^ 1][w4], ((v - 1) >> 1) & 1u, err);
           ok = ok && pr_wait(&pv_done[wg ^ 1], ((v - 1) >> 1) & 1u, err);
           __syncwarp();
           tc_after();
@@ -1238,7 +1247,10 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         tm_wait_st();
         tc_before();
         __syncwarp();
-        if (lane == 0 && ok) arrive_leader<CG>(&p_ready[wg]);
+        if (lane == 0 && ok) {
+          arrive_leader<CG>(&p_ready[wg]);
+          if constexpr (Cfg::kOwnP) mbar_arrive(&pv_seen[wg][w4]);  // the product of tile v - 2 has landed
+        }
       }
       v0 += uint32_t(g.units);
       // ---- the item's sums of this warpgroup's tiles go to the item warps
