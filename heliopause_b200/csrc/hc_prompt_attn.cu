@@ -844,7 +844,9 @@ __global__ void __launch_bounds__(PrCfg<D>::kThreads, 1)
         if (!ok) return;
         tc_after();
         ++ends;
-        const float2 a = s_l[0][rr], b = s_l[1][rr];
+        // the even tiles' sum first, whichever warpgroup had them
+        const uint32_t even = (v0 - uint32_t(g.units)) & 1u;
+        const float2 a = s_l[even][rr], b = s_l[even ^ 1u][rr];
         m = fmaxf(a.x, b.x);
         l = m == -INFINITY ? a.y + b.y : a.y * ex2((a.x - m) * sc) + b.y * ex2((b.x - m) * sc);
         odd = *static_cast<volatile int*>(&s_odd[n & 3]) == n + 1;
