@@ -32,9 +32,9 @@
 // order does not matter).  Chunks are as long as leaves every SM two CTAs, up to
 // 32768 tokens: what a CTA does before and behind the stream, chains of
 // dependent steps of some microseconds, is then paid once.
-// Measured: 64 x 262144 with histories, biases and a mask 44.5 us (69 MB, 1.6
+// Measured: 64 x 262144 with histories, biases and a mask 45.5 us (69 MB, 1.5
 // TB/s; a chunk takes 19 us of such steps and 512 chunks are two rounds of the
-// machine), one row of 262144 9.9 us, two such chains one behind the other.
+// machine), one row of 262144 9.9 to 12 us, two such chains one behind the other.
 #include <algorithm>
 #include <atomic>
 

@@ -35,10 +35,10 @@
 // through scalar sums over the visible pairs.
 //
 // Measured: 32 sequences of 8192 to 32768 keys, 32 / 8 heads of 128 (2.72 GB)
-// 402 us with the join, 6.8 TB/s -- a little above a plain copy's rate; 64 chats
-// of 1 to 4096 keys, 8 / 2 heads of 256 (268 MB) 55 us, 4.9 TB/s: there each CTA
+// 398 to 410 us with the join, 6.7 TB/s -- a little above a plain copy's rate; 64 chats
+// of 1 to 4096 keys, 8 / 2 heads of 256 (268 MB) 52.5 us, 5.1 TB/s: there each CTA
 // has 29 tiles and pays some 12 us of starts, page look-ups, merge and join
-// beside them, which is what one chat's token takes (10.8 us).
+// beside them, which is what one chat's token takes (10.3 to 10.8 us).
 #include <algorithm>
 #include <atomic>
 

@@ -361,7 +361,7 @@ int hpc_prompt_attention(const void *d_q, size_t q_stride, const void *d_k, size
  * ids / vals [rows][k]: value descending, then id ascending, as
  * hpc_sample_candidates takes them.  A token whose value is -inf or NaN is
  * never returned: a row with fewer than k others ends in (-1, -inf) entries.
- * Softcapped logits are capped by the caller before. */
+ * Softcapped logits are capped by the caller before.  At most 65535 rows a call. */
 #define HPC_LOGITS_MAX_VOCAB (1u << 20)
 int hpc_logits_topk_workspace_bytes(size_t rows, size_t vocab, size_t k, size_t *out_bytes);
 int hpc_logits_topk(const float *d_logits, size_t row_stride, size_t rows, size_t vocab, size_t k,
